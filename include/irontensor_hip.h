@@ -505,6 +505,84 @@ it_status it_lion_step(it_context *ctx, int count, float *const *weights, float 
                        const float *const *grads, const int64_t *sizes, float lr, float beta1, float beta2,
                        float weight_decay, const float *grad_scale, const float *lr_dev);
 
+/* ---------------------------------------------------------------- quantised serving
+ *
+ * Decoding with a key/value cache in 4 or 8 bits and weights in 8 bits. No counterpart in the reference,
+ * whose inference recomputes the whole prompt for every token and keeps weights in FP32 or BF16
+ * (src/inference). All calls are stream-ordered like it_gemm, run on the context's device whatever the
+ * current one is, allocate nothing but library scratch (grown once per shape, not during a capture), and
+ * are deterministic.
+ *
+ * Quantising a group of values: step s = max|x| / L with L = 7 (4 bits) or 127 (8 bits), codes = x / s
+ * rounded to nearest even (the real quotient's rounding), value = code * s. A step below 2^-126 is 0 and
+ * the group reads as zeros; a group that holds a NaN or an infinity reads as NaN.
+ */
+
+/* A cache of `capacity` tokens of `batch` sequences with `kv_heads` heads. Keys are quantised in groups of
+ * 32 channels of a token and head, values in one group per token and head; steps are rounded to BF16 (and
+ * codes chosen for the rounded step). `data`: it_kv_cache_bytes() bytes, 16-byte aligned, in a layout of
+ * the library's own, to be zeroed (it_zero) before first use; the caller owns it. A copy of those bytes is a
+ * copy of the cache. */
+typedef struct it_kv_cache {
+    int bits;          /* 4 or 8 */
+    int64_t batch, kv_heads, capacity;
+    int64_t head_dim;  /* 64, 128 or 256 (IT_ERR_DIMS otherwise) */
+    void *data;
+} it_kv_cache;
+
+/* Bytes of a cache's data (bits / 8 bytes a value and 2 bytes a step, tokens rounded up to 64). One head of
+ * a sequence must stay below 2 GiB (IT_ERR_DIMS). */
+it_status it_kv_cache_bytes(int bits, int64_t batch, int64_t kv_heads, int64_t capacity, int64_t head_dim,
+                            size_t *bytes);
+
+/* Quantises token i < count[b] of K and V ([batch, kv_heads] rows of n tokens through kv_layout; FP32 or
+ * BF16) into position start[b] + i of sequence b. start, count: device int32 [batch]; count NULL: n of
+ * every sequence. Tokens whose position is outside [0, capacity) are not written; no other position of the
+ * cache changes. kv_layout NULL: [batch, kv_heads, n, head_dim] contiguous. */
+it_status it_kv_cache_write(it_context *ctx, it_dtype dtype, const it_kv_cache *cache, int64_t n,
+                            const it_attn_layout *kv_layout, const void *K, const void *V, const int32_t *start,
+                            const int32_t *count);
+
+/* The values that positions begin .. begin + n - 1 of every sequence stand for (code * step, one rounding
+ * to dtype) into K and V through kv_layout (NULL: [batch, kv_heads, n, head_dim] contiguous); positions never
+ * written read as 0. begin + n may not pass the capacity (IT_ERR_SHAPE). */
+it_status it_kv_cache_read(it_context *ctx, it_dtype dtype, const it_kv_cache *cache, int64_t begin, int64_t n,
+                           const it_attn_layout *kv_layout, void *K, void *V);
+
+/* Attention of n queries of every sequence over its cached tokens: query i < count[b] of sequence b stands
+ * at position start[b] + i and sees the positions up to its own, O = softmax(scale Q.K^T).V on the values
+ * that the cache stands for. Its own token is written first (it_kv_cache_write with the same start and
+ * count): n == 1 is a decoding step, larger n a piece of a prompt. A query with i >= count[b], or that sees
+ * no position, gets zeros; positions at the capacity and beyond are not seen. Positions that a query does not
+ * see do not reach its result, whatever they hold.
+ * heads: a multiple of the cache's; head h reads cache head h / (heads / kv_heads). Q, O: FP32 or BF16,
+ * [batch, heads, n, head_dim] contiguous or through q_layout and o_layout (NULL: q_layout), strides and
+ * alignment as they come (16-byte multiples are faster). scale finite and > 0. FP32 results carry FP32
+ * accuracy for the values the cache stands for; with BF16, probabilities are rounded to BF16 before their
+ * product with the values. */
+it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache *cache, int64_t heads, int64_t n,
+                              float scale, const it_attn_layout *q_layout, const it_attn_layout *o_layout,
+                              const void *Q, const int32_t *start, const int32_t *count, void *O);
+
+/* Rows of X [rows, cols] (FP32 or BF16, leading dimension ldx) as 8-bit codes [rows, ldc] and one FP32 step a
+ * row (a weight's output channels, or tokens). ldc: a multiple of 16, at least cols; codes from cols to the
+ * next multiple of 16 are written as 0. codes 16-byte aligned. */
+it_status it_quantize_i8(it_context *ctx, it_dtype dtype, int64_t rows, int64_t cols, const void *X, int64_t ldx,
+                         int8_t *codes, int64_t ldc, float *steps);
+
+/* C[m, n] = (sum_k A[m, k] B[n, k]) steps_a[m] steps_b[n] + bias[n] in FP32 or BF16: A [M, K] and B [N, K]
+ * 8-bit codes, exact 32-bit sums. K a multiple of 16, at most 131056; lda, ldb multiples of 16, at most
+ * 4194304; codes 16-byte aligned; bias NULL: none. */
+it_status it_gemm_i8(it_context *ctx, it_dtype dtype_out, int64_t M, int64_t N, int64_t K, const int8_t *A, int64_t lda,
+                     const float *steps_a, const int8_t *B, int64_t ldb, const float *steps_b, const float *bias, void *C,
+                     int64_t ldc);
+
+/* A linear layer on an 8-bit weight: Y = X.W^T + bias with X [M, K] quantised per row as it_quantize_i8 does
+ * (into library scratch) and W [N, K] codes from it_quantize_i8 (padded with zeros to a multiple of 16).
+ * X and Y in dtype. Any K up to 131056. */
+it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, int64_t K, const void *X, int64_t ldx,
+                       const int8_t *W, int64_t ldw, const float *steps_w, const float *bias, void *Y, int64_t ldy);
+
 /* ---------------------------------------------------------------- synthetic inputs */
 
 /*

@@ -13,5 +13,7 @@ from .ops import (Linear, attention, attention_backward_recompute, attention_for
                   matmul_bf16_batched, matmul_custom, matmul_mps, matmul_mps_nt, matmul_mps_tn,
                   matmul_tn, softmax_backward, softmax_rows, swiglu_up, to_bf16_gpu, to_f32_gpu,
                   causal_mask_3d_gpu, transpose_3d_gpu)
+from .quant_ops import (Int8Matrix, KvCache, LinearI8, Positions, cached_attention, kv_cache_read, kv_cache_write,
+                        linear_i8, matmul_i8, quantize_i8, upload_positions)
 
 __all__ = [name for name in dir() if not name.startswith("_")]

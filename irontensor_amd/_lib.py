@@ -92,6 +92,17 @@ class AttnLayout(C.Structure):
     ]
 
 
+class KvCacheDesc(C.Structure):
+    _fields_ = [
+        ("bits", c_int),
+        ("batch", c_i64),
+        ("kv_heads", c_i64),
+        ("capacity", c_i64),
+        ("head_dim", c_i64),
+        ("data", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "it_init": (c_int, [c_int, C.POINTER(c_void_p)]),
@@ -181,6 +192,19 @@ _SIGNATURES = {
                                               c_void_p, c_void_p, c_void_p, c_void_p, c_i64]),
     "it_transpose_3d": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64]),
     "it_causal_mask_3d": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_i64]),
+    "it_kv_cache_bytes": (c_int, [c_int, c_i64, c_i64, c_i64, c_i64, C.POINTER(C.c_size_t)]),
+    "it_kv_cache_write": (c_int, [c_void_p, c_int, C.POINTER(KvCacheDesc), c_i64, C.POINTER(AttnLayout), c_void_p,
+                                  c_void_p, c_void_p, c_void_p]),
+    "it_kv_cache_read": (c_int, [c_void_p, c_int, C.POINTER(KvCacheDesc), c_i64, c_i64, C.POINTER(AttnLayout), c_void_p,
+                                 c_void_p]),
+    "it_cached_attention": (c_int, [c_void_p, c_int, C.POINTER(KvCacheDesc), c_i64, c_i64, c_float,
+                                    C.POINTER(AttnLayout), C.POINTER(AttnLayout), c_void_p, c_void_p, c_void_p,
+                                    c_void_p]),
+    "it_quantize_i8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p]),
+    "it_gemm_i8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_void_p,
+                           c_void_p, c_void_p, c_i64]),
+    "it_linear_i8": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p,
+                             c_void_p, c_i64]),
     "it_fill_normal": (c_int, [c_void_p, c_int, C.c_uint64, c_i64, c_i64, C.c_double, c_void_p]),
     "it_side_begin": (c_int, [c_void_p]),
     "it_side_end": (c_int, [c_void_p]),

@@ -25,7 +25,8 @@ TUNING_LIB = PKG / "libirontensor_hip_tuning.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["runtime.cpp", "api.cpp", "api_train.cpp", "kernels_gemm.hip", "kernels_gemm_f32.hip", "kernels_misc.hip",
-           "kernels_flash.hip", "kernels_gemv.hip", "kernels_train.hip", "noalloc.hip", "kernels_flash2.hip"]
+           "kernels_flash.hip", "kernels_gemv.hip", "kernels_train.hip", "noalloc.hip", "kernels_flash2.hip",
+           "api_quant.cpp", "kernels_cache.hip", "kernels_cached_attn.hip", "kernels_i8.hip"]
 #: Sources with planner overrides (IT_TUNING).
 TUNED = ["kernels_gemm.hip", "kernels_gemm_f32.hip"]
 

@@ -1,0 +1,123 @@
+// What the 8- and 4-bit operators share: the quantiser, the layout of the key/value cache, and the
+// arguments of their launches.
+#pragma once
+
+#include "internal.hpp"
+#include "mfma.hpp"
+
+namespace it {
+
+// ------------------------------------------------------------------ the quantiser
+
+// A group of values shares the step s = max|x| / L (L: the largest code) and keeps n = rne(x / s). A step
+// below the smallest normal number is stored as 0 (the group reads as zeros); a group that holds a NaN or
+// an infinity gets s = NaN and codes 0, so that all of it reads as NaN.
+constexpr float QUANT_TINY = 1.17549435e-38f;  // 2^-126
+
+// The step from the largest |x|, given as its bits (compared as integers they order NaN above infinity
+// above every number, so one integer maximum finds non-finite values too). BF16: the cache's steps are
+// rounded to BF16, whose 8 significand bits cost nothing: codes are chosen for the step as stored. L times
+// its rounding error stays below half a step for L = 7; for L = 127 a quotient up to 127.5 is clamped.
+template <bool BF16>
+__device__ __forceinline__ float quant_step(uint32_t maxbits, float levels) {
+    if (maxbits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    float s = __uint_as_float(maxbits) / levels;
+    if constexpr (BF16) s = bf16_to_f32(f32_to_bf16_rne(s));
+    return s < QUANT_TINY ? 0.f : s;
+}
+
+// 1 / s, or 0 where every code is 0.
+__device__ __forceinline__ float quant_inverse(float s) { return s > 0.f ? 1.f / s : 0.f; }
+
+// rne(x / s) of the real quotient, clamped to +-levels. x * inv is within 2^-22 of the quotient's value, so
+// its nearest whole number n is off by at most one, and only where the quotient is next to a half. The
+// rest x - n s is exact in one FMA (its bits lie between ulp(x) and s), and so is its comparison with s / 2:
+// above it the code is the next one, at it the even one.
+__device__ __forceinline__ float quant_code(float x, float s, float inv, float levels) {
+    float n = rintf(x * inv);
+    const float r = fmaf(-n, s, x), h = 0.5f * s, a = fabsf(r);
+    const bool odd = ((int)n & 1) != 0;
+    if (inv > 0.f && (a > h || (a == h && odd))) n += copysignf(1.f, r);
+    return fminf(fmaxf(n, -levels), levels);
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// ------------------------------------------------------------------ the cache
+
+// One region for each (sequence, head): key codes, value codes, key steps, value steps, all BF16 steps.
+// T = capacity rounded up to CACHE_TILE tokens, R = head_dim * bits / 8 bytes of codes a token:
+//   key codes    [T][R]: a token's row holds, for lane group g = 0..3 of an MFMA operand, channels
+//                32 s + 8 g .. + 7 of s = 0, 1, ..: a lane's operands of every 32-channel step are
+//                consecutive bytes. In 4 bits the eight codes of an octet are one word, even channel e at
+//                nibble e / 2 and odd e at nibble e / 2 + 4, so that a shift and a mask give pairs.
+//   value codes  [T / 4][head_dim / 4][4 tokens][4 codes] in 4 bits, [T / 4][head_dim][4 tokens] in 8: the
+//                four tokens that a lane's operand needs of a channel are together, and a token's codes are
+//                whole bytes of their own (2, or 1), so appending one rewrites nobody else's.
+//   key steps    [T][head_dim / 32], value steps [T].
+// Codes are stored biased by 8 (128): an all-zero region reads as zeros, its steps being zero.
+constexpr int64_t CACHE_TILE = 64;
+constexpr int CACHE_GROUP = 32;
+
+struct CacheGeom {
+    char *data;
+    int64_t region;                   // bytes of one (sequence, head)
+    int64_t v_off, ks_off, vs_off;    // value codes, key steps and value steps within it
+    int64_t capacity;
+    int64_t batch, kv_heads;
+    int bits, head_dim;
+};
+
+// Per-head addressing of a 16- or 32-bit operand: (bh / heads) * bs + (bh % heads) * hs + row * rs + d.
+struct HeadLayout {
+    int64_t heads, bs, hs, rs;
+    __host__ __device__ int64_t at(int64_t bh) const { return (bh / heads) * bs + (bh % heads) * hs; }
+};
+
+struct CacheMoveArgs {
+    CacheGeom c;
+    const void *K, *V;      // written from
+    void *Ko, *Vo;          // read into
+    HeadLayout lay;
+    const int32_t *start, *count;
+    int64_t begin, n;
+    int64_t blocks;         // 4-token blocks of a (sequence, head) that the call may touch
+    int vec_ok;             // rows allow 16-byte accesses
+};
+it_status launch_cache_write(hipStream_t s, bool bf16, const CacheMoveArgs &a);
+it_status launch_cache_read(hipStream_t s, bool bf16, const CacheMoveArgs &a);
+
+struct CachedAttnArgs {
+    CacheGeom c;
+    const void *Q;
+    void *O;
+    HeadLayout ql, ol;
+    const int32_t *start, *count;
+    int64_t heads, n;       // query heads; queries of a sequence
+    int share;              // query heads of one cache head
+    int rows;               // n * share
+    int row_blocks, splits;
+    float scale_log2;       // scale * log2 e
+    float *part;            // splits > 1: partial results, and
+    int *counters;          // one arrival counter for each (sequence, head, row block)
+    int q_vec, o_vec;
+};
+// Fills in row_blocks and splits; the floats of `part` that the launch then needs (0: none).
+int64_t plan_cached_attention(CachedAttnArgs &a, bool bf16, int num_cus);
+it_status launch_cached_attention(hipStream_t s, bool bf16, const CachedAttnArgs &a);
+
+// ------------------------------------------------------------------ 8-bit products
+
+struct GemmI8Args {
+    const int8_t *A, *B;            // [M, K], [N, K]
+    const float *sA, *sB, *bias;    // [M], [N], [N] or NULL
+    void *C;
+    int64_t M, N, K, lda, ldb, ldc;
+    int out_bf16;
+    int tiles_m, tiles_n;
+};
+it_status launch_quantize_i8(hipStream_t s, bool bf16, int64_t rows, int64_t cols, const void *X, int64_t ldx,
+                             int8_t *codes, int64_t ldc, float *steps);
+it_status launch_gemm_i8(it_context *ctx, GemmI8Args a);
+
+}  // namespace it

@@ -1,0 +1,76 @@
+"""The quantised serving operators in 64 bits, from their definition, for the tests of them."""
+from __future__ import annotations
+
+import numpy as np
+
+from irontensor_amd.tensor import bf16_to_f32, f32_to_bf16
+
+TINY = 2.0 ** -126
+GROUP = 32
+
+
+def rne_bf16(x):
+    return bf16_to_f32(f32_to_bf16(np.asarray(x, np.float32))).reshape(np.shape(x))
+
+
+def steps(x, group, levels, bf16=True):
+    """[.., D / group] FP32 steps of x [.., D]: max|x| / levels, NaN where a value is not finite."""
+    g = np.asarray(x, np.float32).reshape(*x.shape[:-1], x.shape[-1] // group, group)
+    with np.errstate(invalid="ignore"):
+        most = np.abs(g).max(-1)
+    s = most / np.float32(levels)
+    if bf16:
+        s = rne_bf16(s)
+    s = np.where(s < TINY, np.float32(0), s)
+    return np.where(np.isfinite(g).all(-1), s, np.float32(np.nan))
+
+
+def codes(x, s, group, levels):
+    """rne(x / s) in float64 (a quotient of two FP32 numbers of which one has at most 32 bits times a half
+    is never mistaken there), 0 where the step is 0 or NaN."""
+    g = np.asarray(x, np.float64).reshape(*x.shape[:-1], x.shape[-1] // group, group)
+    live = s > 0
+    with np.errstate(invalid="ignore", divide="ignore"):
+        q = np.rint(g / np.where(live, s, 1).astype(np.float64)[..., None])
+    return np.where(live[..., None], np.clip(q, -levels, levels), 0).reshape(x.shape)
+
+
+def stands_for(x, group, levels, bf16=True):
+    s = steps(x, group, levels, bf16)
+    return codes(x, s, group, levels) * np.repeat(s.astype(np.float64), group, -1)
+
+
+def cache_values(k, v, bits):
+    """What keys and values [.., D] read back as."""
+    levels = 7 if bits == 4 else 127
+    return stands_for(k, GROUP, levels), stands_for(v, v.shape[-1], levels)
+
+
+def attend(q, k, v, start, count, scale, capacity=None):
+    """(o, sum p|v|, largest scale * sum|q k| of a row) of q [B, n, H, D] over k, v [B, T, Hkv, D] in float64."""
+    b, n, h, d = q.shape
+    t, hkv = k.shape[1:3]
+    o, pv, mag = (np.zeros(q.shape), np.zeros(q.shape), np.zeros((b, n, h)))
+    for bi in range(b):
+        for i in range(min(n, max(0, int(count[bi])))):
+            lim = min(max(int(start[bi]) + i + 1, 0), t)
+            if lim == 0:
+                continue
+            for hi in range(h):
+                kk, vv = k[bi, :lim, hi // (h // hkv)], v[bi, :lim, hi // (h // hkv)]
+                x = q[bi, i, hi].astype(np.float64)
+                s = kk @ x * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                o[bi, i, hi], pv[bi, i, hi] = p @ vv, p @ np.abs(vv)
+                mag[bi, i, hi] = (np.abs(kk) @ np.abs(x)).max() * scale
+    return o, pv, mag
+
+
+def attend_bound(o, pv, mag, t, d, bf16):
+    """Largest error of an element. FP32: a score is an FP32 sum of D products and D / 32 multiples of them, off by
+    at most (D + 16) 2^-24 of the sum of their magnitudes; 2^x is off by 2^-21 for the sizes of x here, the
+    scaled exponent's rounding among it (2^-24 |x|, |x| < 2^3 mag); a numerator and a denominator carry that,
+    and sums of T terms, each off by at most T 2^-24. BF16: P rounded (2^-8 a term) and the output (2^-8)."""
+    e = 2 * ((d + 16 + 8) * 2.0 ** -24 * mag[..., None] + 2.0 ** -21 + t * 2.0 ** -24) * pv
+    return e + (2.0 ** -8 * (pv + np.abs(o) + e) if bf16 else 2.0 ** -24 * np.abs(o))
