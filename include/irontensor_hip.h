@@ -566,20 +566,20 @@ it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache
 
 /* Rows of X [rows, cols] (FP32 or BF16, leading dimension ldx) as 8-bit codes [rows, ldc] and one FP32 step a
  * row (a weight's output channels, or tokens). ldc: a multiple of 16, at least cols; codes from cols to the
- * next multiple of 16 are written as 0. codes 16-byte aligned. */
+ * next multiple of 128 (to ldc, if that is less) are written as 0. codes 16-byte aligned. */
 it_status it_quantize_i8(it_context *ctx, it_dtype dtype, int64_t rows, int64_t cols, const void *X, int64_t ldx,
                          int8_t *codes, int64_t ldc, float *steps);
 
 /* C[m, n] = (sum_k A[m, k] B[n, k]) steps_a[m] steps_b[n] + bias[n] in FP32 or BF16: A [M, K] and B [N, K]
- * 8-bit codes, exact 32-bit sums. K a multiple of 16, at most 131056; lda, ldb multiples of 16, at most
- * 4194304; codes 16-byte aligned; bias NULL: none. */
+ * 8-bit codes, exact 32-bit sums. K a multiple of 16 (128: faster), at most 131056; lda, ldb multiples of
+ * 16, at most 4194304; codes 16-byte aligned; bias NULL: none. */
 it_status it_gemm_i8(it_context *ctx, it_dtype dtype_out, int64_t M, int64_t N, int64_t K, const int8_t *A, int64_t lda,
                      const float *steps_a, const int8_t *B, int64_t ldb, const float *steps_b, const float *bias, void *C,
                      int64_t ldc);
 
 /* A linear layer on an 8-bit weight: Y = X.W^T + bias with X [M, K] quantised per row as it_quantize_i8 does
- * (into library scratch) and W [N, K] codes from it_quantize_i8 (padded with zeros to a multiple of 16).
- * X and Y in dtype. Any K up to 131056. */
+ * (into library scratch) and W [N, K] codes from it_quantize_i8, padded with zeros to a multiple of 16, or of
+ * 128 where ldw has the room. X and Y in dtype. Any K up to 130944. */
 it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, int64_t K, const void *X, int64_t ldx,
                        const int8_t *W, int64_t ldw, const float *steps_w, const float *bias, void *Y, int64_t ldy);
 

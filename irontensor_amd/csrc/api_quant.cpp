@@ -158,7 +158,6 @@ it_status it_kv_cache_write(it_context *ctx, it_dtype dtype, const it_kv_cache *
         a.blocks = n > MAX_DIM ? MAX_DIM : (n + 3 + 3) / 4;
         if (a.blocks > MAX_GRID || a.c.batch * a.c.kv_heads > MAX_GRID / a.blocks)
             return fail(IT_ERR_DIMS, std::string(op) + ": too many tokens");
-        a.vec_ok = vec16(K, a.lay, esize(dtype)) && (uintptr_t)V % 16 == 0;
         const OnDevice dev(ctx);
         return profiled(
             ctx, [&] { return "kv_write" + i64(a.c.bits) + "[" + i64(a.c.batch * a.c.kv_heads) + "x" + i64(n) + "x" + i64(a.c.head_dim) + "]"; },
@@ -186,7 +185,6 @@ it_status it_kv_cache_read(it_context *ctx, it_dtype dtype, const it_kv_cache *c
         a.n = n;
         a.blocks = (begin % 4 + n + 3) / 4;
         if (a.c.batch * a.c.kv_heads > MAX_GRID / a.blocks) return fail(IT_ERR_DIMS, std::string(op) + ": too many tokens");
-        a.vec_ok = vec16(K, a.lay, esize(dtype)) && (uintptr_t)V % 16 == 0;
         const OnDevice dev(ctx);
         return profiled(
             ctx, [&] { return "kv_read" + i64(a.c.bits) + "[" + i64(a.c.batch * a.c.kv_heads) + "x" + i64(n) + "x" + i64(a.c.head_dim) + "]"; },
@@ -290,7 +288,7 @@ it_status it_gemm_i8(it_context *ctx, it_dtype dtype_out, int64_t M, int64_t N, 
         if (const it_status st = check_gemm_i8(op, M, N, K, A, lda, steps_a, B, ldb, steps_b, C, ldc); st != IT_OK) return st;
         if (M == 0 || N == 0) return IT_OK;
         const OnDevice dev(ctx);
-        const it::GemmI8Args a{A, B, steps_a, steps_b, bias, C, M, N, K, lda, ldb, ldc, dtype_out == IT_BF16, 0, 0};
+        const it::GemmI8Args a{A, B, steps_a, steps_b, bias, C, M, N, K, lda, ldb, ldc, dtype_out == IT_BF16, 0, 0, nullptr, 0, 0};
         return profiled(
             ctx, [&] { return "gemm_i8[" + i64(M) + "x" + i64(N) + "x" + i64(K) + "]"; },
             [&] { return it::launch_gemm_i8(ctx, a); });
@@ -303,8 +301,11 @@ it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, in
     return guarded(op, [&]() -> it_status {
         if (!ctx) return fail(IT_ERR_NULL, std::string(op) + ": ctx is NULL");
         if (!f32_or_bf16(dtype)) return bad_dtype(op);
-        if (K < 0 || K > MAX_K) return check_gemm_i8(op, M, N, K, nullptr, 0, nullptr, nullptr, 0, nullptr, nullptr, 0);
-        const int64_t kp = (K + 15) / 16 * 16;
+        const int64_t max_k = MAX_K / 128 * 128;
+        if (K > max_k) return fail(IT_ERR_DIMS, std::string(op) + ": K must be at most " + i64(max_k) + " (32-bit sums), got " + i64(K));
+        if (K < 0) return check_gemm_i8(op, M, N, K, nullptr, 0, nullptr, nullptr, 0, nullptr, nullptr, 0);
+        // Whole k-tiles of 128 where the weight's rows have them (it_quantize_i8 pads rows that far).
+        const int64_t k128 = (K + 127) / 128 * 128, kp = ldw >= k128 ? k128 : (K + 15) / 16 * 16;
         // The activations' codes go to scratch: 16 is any non-NULL aligned address for the check.
         if (const it_status st = check_gemm_i8(op, M, N, kp, (const int8_t *)16, kp, (const float *)16, W, ldw, steps_w, Y, ldy); st != IT_OK) return st;
         if (ldx < K || ldx > MAX_DIM) return fail(IT_ERR_INVALID, std::string(op) + ": ldx smaller than K");
@@ -312,6 +313,12 @@ it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, in
         if (K > 0 && !X) return fail(IT_ERR_NULL, std::string(op) + ": NULL buffer");
         if (M > MAX_GRID) return fail(IT_ERR_DIMS, std::string(op) + ": matrix too large");
         const OnDevice dev(ctx);
+        if (it::gemv_i8_x_applicable(M, kp)) {
+            const it::GemmI8Args a{nullptr, W, nullptr, steps_w, bias, Y, M, N, kp, kp, ldw, ldy, dtype == IT_BF16, 0, 0, X, ldx, (int)K};
+            return profiled(
+                ctx, [&] { return "linear_i8[" + i64(M) + "x" + i64(N) + "x" + i64(K) + "]"; },
+                [&] { return it::launch_gemv_i8_x(ctx->stream, dtype == IT_BF16, a); });
+        }
         const size_t steps_at = ((size_t)(M * kp) + 255) / 256 * 256;
         void *ws = nullptr;
         if (const it_status st = it::ensure_scratch(ctx, steps_at + (size_t)M * sizeof(float), &ws); st != IT_OK) return st;
@@ -321,7 +328,7 @@ it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, in
             ctx, [&] { return "quantize_i8[" + i64(M) + "x" + i64(K) + "]"; },
             [&] { return it::launch_quantize_i8(ctx->stream, dtype == IT_BF16, M, K, X, ldx, codes, kp, steps); });
         if (qs != IT_OK) return qs;
-        const it::GemmI8Args a{codes, W, steps, steps_w, bias, Y, M, N, kp, kp, ldw, ldy, dtype == IT_BF16, 0, 0};
+        const it::GemmI8Args a{codes, W, steps, steps_w, bias, Y, M, N, kp, kp, ldw, ldy, dtype == IT_BF16, 0, 0, nullptr, 0, 0};
         return profiled(
             ctx, [&] { return "gemm_i8[" + i64(M) + "x" + i64(N) + "x" + i64(K) + "]"; },
             [&] { return it::launch_gemm_i8(ctx, a); });

@@ -15,50 +15,63 @@ namespace {
 
 constexpr int CM_THREADS = 256;
 
+// Vector accesses that need an element's alignment only.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// Eight channels as loaded.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, int vec_ok, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec_ok) {
-            const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 4);
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
-        } else {
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const u32x4 v = *(const u32x4_any *)((const char *)p + 16 * i);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = p[e];
-        }
-    } else {
-        if (vec_ok) {
-            const u32x4 h = *(const u32x4 *)p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[2 * e] = __uint_as_float(h[e] << 16);
-                x[2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = bf16_to_f32(p[e]);
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
         }
     }
-}
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
+    }
+    // Bits of the largest |x|.
+    __device__ __forceinline__ uint32_t most() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = max(m, w[e] & 0x7fffffffu);
+            return m;
+        } else {
+            // two to a word: the high halves compare as the words they begin, the low ones shifted up
+            uint32_t hi = 0, lo = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                hi = max(hi, w[e] & 0x7fff0000u);
+                lo = max(lo, w[e] & 0x7fffu);
+            }
+            return max(hi, lo << 16);
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (sizeof(T) == 4)
+                x[e] = __uint_as_float(w[e]);
+            else
+                x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        }
+    }
+};
 
 template <typename T>
-__device__ __forceinline__ void store8(T *p, int vec_ok, const float (&x)[8]) {
+__device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
-        if (vec_ok) {
-            *(f32x4 *)p = f32x4{x[0], x[1], x[2], x[3]};
-            *(f32x4 *)(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = x[e];
-        }
+        *(f32x4_any *)p = f32x4{x[0], x[1], x[2], x[3]};
+        *(f32x4_any *)(p + 4) = f32x4{x[4], x[5], x[6], x[7]};
     } else {
-        if (vec_ok) {
-            *(u32x4 *)p = u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+        *(u32x4_any *)p = u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
                                 pack_bf16x2(x[6], x[7])};
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = f32_to_bf16_rne(x[e]);
-        }
     }
 }
 
@@ -70,13 +83,6 @@ __device__ __forceinline__ uint32_t max_over(uint32_t v) {
         v = v > w ? v : w;
     }
     return v;
-}
-
-__device__ __forceinline__ uint32_t max8(const float (&x)[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, abs_bits(x[e]));
-    return m;
 }
 
 // Nibble of channel e of an octet in a key word.
@@ -101,7 +107,7 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
     const int64_t pb = ((p0 >> 2) + blk) * 4;
     const T *Kp = (const T *)p.K + p.lay.at(bh) + 8 * c, *Vp = (const T *)p.V + p.lay.at(bh) + 8 * c;
     char *region = p.c.data + bh * p.c.region;
-    float kx[4][8], vx[4][8];
+    Raw8<T> kx[4], vx[4];
     bool ok[4];
     int some = 0, all = 1;
 #pragma unroll
@@ -111,65 +117,66 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
         some |= ok[t];
         all &= ok[t];
         if (ok[t]) {
-            load8(Kp + i * p.lay.rs, p.vec_ok, kx[t]);
-            load8(Vp + i * p.lay.rs, p.vec_ok, vx[t]);
+            kx[t].load(Kp + i * p.lay.rs);
+            vx[t].load(Vp + i * p.lay.rs);
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) kx[t][e] = vx[t][e] = 0.f;
+            kx[t].zero();
+            vx[t].zero();
         }
     }
-    float vn[4][8];
+    const int s = c / 4, g = c % 4;
+    uint32_t vu[4][8];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const float ks = quant_step<true>(max_over<4>(max8(kx[t])), L), ki = quant_inverse(ks);
-        const float vs = quant_step<true>(max_over<OCT>(max8(vx[t])), L), vi = quant_inverse(vs);
-        float kn[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            kn[e] = ki > 0.f ? quant_code(kx[t][e], ks, ki, L) : 0.f;
-            vn[t][e] = vi > 0.f ? quant_code(vx[t][e], vs, vi, L) : 0.f;
-        }
+        const float ks = quant_step<true>(max_over<4>(kx[t].most()), L), ki = quant_inverse(ks);
+        const float vs = quant_step<true>(max_over<OCT>(vx[t].most()), L), vi = quant_inverse(vs);
+        float x[8];
+        uint32_t ku[8];
+        kx[t].values(x);
+        quant_codes<BIAS>(x, ks, ki, ku);
+        vx[t].values(x);
+        quant_codes<BIAS>(x, vs, vi, vu[t]);
         if (!ok[t]) continue;
         const int64_t pos = pb + t;
-        const int s = c / 4, g = c % 4;
         char *kd = region + pos * ROW + g * (ROW / 4);
         if constexpr (BITS == 4) {
-            uint32_t w = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w |= (uint32_t)((int)kn[e] + BIAS) << (4 * key_nibble(e));
-            *(uint32_t *)(kd + 4 * s) = w;
+            // key_nibble: bytes of channels (0, 2), (4, 6), (1, 3), (5, 7)
+            *(uint32_t *)(kd + 4 * s) = bytes4(ku[0], ku[4], ku[1], ku[5]) | bytes4(ku[2], ku[6], ku[3], ku[7]) << 4;
         } else {
-            u32x2 w = {0u, 0u};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)((int)kn[e] + BIAS) << (8 * (e & 3));
-            *(u32x2 *)(kd + 8 * s) = w;
+            *(u32x2 *)(kd + 8 * s) = u32x2{bytes4(ku[0], ku[1], ku[2], ku[3]), bytes4(ku[4], ku[5], ku[6], ku[7])};
         }
         if (g == 0) *(uint16_t *)(region + p.c.ks_off + (pos * (D / CACHE_GROUP) + s) * 2) = f32_to_bf16_rne(ks);
         if (c == 0) *(uint16_t *)(region + p.c.vs_off + pos * 2) = f32_to_bf16_rne(vs);
     }
     if (!some) return;
     constexpr int WORDS = BITS;  // 8 channels of four tokens
-    uint32_t w[WORDS], keep[WORDS];
+    uint32_t w[WORDS];
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) w[i] = keep[i] = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t u = (uint32_t)((int)vn[t][e] + BIAS);
-            const int i = BITS == 4 ? 2 * (e / 4) + t / 2 : e;
-            const int sh = BITS == 4 ? 16 * (t & 1) + 4 * (e & 3) : 8 * t;
-            w[i] |= ok[t] ? u << sh : 0u;
-            keep[i] |= ok[t] ? 0u : (BITS == 4 ? 15u : 255u) << sh;
+    for (int i = 0; i < WORDS; ++i) {
+        if constexpr (BITS == 4) {
+            const int e = 4 * (i / 2), t = 2 * (i & 1);
+            w[i] = bytes4(vu[t][e], vu[t][e + 2], vu[t + 1][e], vu[t + 1][e + 2]) |
+                   bytes4(vu[t][e + 1], vu[t][e + 3], vu[t + 1][e + 1], vu[t + 1][e + 3]) << 4;
+        } else {
+            w[i] = bytes4(vu[0][i], vu[1][i], vu[2][i], vu[3][i]);
         }
+    }
     u32x4 *vd = (u32x4 *)(region + p.c.v_off + (pb / 4) * (4 * ROW) + c * (4 * WORDS));
 #pragma unroll
     for (int q = 0; q < WORDS / 4; ++q) {
         u32x4 v = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
         if (!all) {
+            // the other tokens' halves (bytes) of every word stay
             const u32x4 old = vd[q];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] |= old[i] & keep[4 * q + i];
+            for (int i = 0; i < 4; ++i) {
+                uint32_t mine;
+                if constexpr (BITS == 4)
+                    mine = (ok[2 * (i & 1)] ? 0xffffu : 0u) | (ok[2 * (i & 1) + 1] ? 0xffff0000u : 0u);
+                else
+                    mine = (ok[0] ? 0xffu : 0u) | (ok[1] ? 0xff00u : 0u) | (ok[2] ? 0xff0000u : 0u) | (ok[3] ? 0xff000000u : 0u);
+                v[i] = (v[i] & mine) | (old[i] & ~mine);
+            }
         }
         vd[q] = v;
     }
@@ -219,8 +226,8 @@ __global__ __launch_bounds__(CM_THREADS) void cache_read(const CacheMoveArgs p) 
             vx[e] = (float)((int)vu - BIAS) * vs + 0.f;
         }
         const int64_t i = pos - p.begin;
-        store8(Ko + i * p.lay.rs, p.vec_ok, kx);
-        store8(Vo + i * p.lay.rs, p.vec_ok, vx);
+        store8(Ko + i * p.lay.rs, kx);
+        store8(Vo + i * p.lay.rs, vx);
     }
 }
 

@@ -29,16 +29,46 @@ __device__ __forceinline__ float quant_step(uint32_t maxbits, float levels) {
 // 1 / s, or 0 where every code is 0.
 __device__ __forceinline__ float quant_inverse(float s) { return s > 0.f ? 1.f / s : 0.f; }
 
-// rne(x / s) of the real quotient, clamped to +-levels. x * inv is within 2^-22 of the quotient's value, so
-// its nearest whole number n is off by at most one, and only where the quotient is next to a half. The
-// rest x - n s is exact in one FMA (its bits lie between ulp(x) and s), and so is its comparison with s / 2:
-// above it the code is the next one, at it the even one.
-__device__ __forceinline__ float quant_code(float x, float s, float inv, float levels) {
-    float n = rintf(x * inv);
-    const float r = fmaf(-n, s, x), h = 0.5f * s, a = fabsf(r);
-    const bool odd = ((int)n & 1) != 0;
-    if (inv > 0.f && (a > h || (a == h && odd))) n += copysignf(1.f, r);
-    return fminf(fmaxf(n, -levels), levels);
+// Codes of eight values: the low byte of u[e] is rne(x[e] / s) + BIAS of the real quotient (BIAS even).
+// x * inv + 3 2^22 rounds to the nearest whole number n in one FMA, off by at most one and only where the
+// quotient is next to a half. The rest x - n s is exact in one FMA (its bits lie between ulp(x) and s), and so
+// is its comparison with s / 2: above it the code is the next one, at it the even one. That repair is a
+// branch that FP32 values hardly ever take and BF16 ones, which hit halves exactly, in every third pair of a
+// wave. A quotient never passes the largest code L by a half: s is within 2^-8 (BF16) of max|x| / L, and
+// 127 / (1 - 2^-8) < 127.5.
+template <int BIAS>
+__device__ __forceinline__ void quant_codes(const float (&x)[8], float s, float inv, uint32_t (&u)[8]) {
+    constexpr float MAGIC = 12582912.f + BIAS;  // 3 2^22 + BIAS
+    const bool live = inv > 0.f;
+    const float h = live ? 0.5f * s : INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float t[2], r[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            t[i] = fmaf(x[e + i], inv, MAGIC);
+            r[i] = fmaf(MAGIC - t[i], s, x[e + i]);
+        }
+        if (__any(fmaxf(fabsf(r[0]), fabsf(r[1])) >= h)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float a = fabsf(r[i]);
+                if (a > h || (a == h && (__float_as_uint(t[i]) & 1u))) t[i] += copysignf(1.f, r[i]);
+            }
+        }
+        u[e] = __float_as_uint(t[0]);
+        u[e + 1] = __float_as_uint(t[1]);
+    }
+    if (__any(!live)) {  // a group without a step: infinities times 0 must not leave codes
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = live ? u[e] : (uint32_t)BIAS;
+    }
+}
+
+// The low bytes of a, b, c, d, first to last.
+__device__ __forceinline__ uint32_t bytes4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), cd = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+    return ab | cd;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -82,7 +112,6 @@ struct CacheMoveArgs {
     const int32_t *start, *count;
     int64_t begin, n;
     int64_t blocks;         // 4-token blocks of a (sequence, head) that the call may touch
-    int vec_ok;             // rows allow 16-byte accesses
 };
 it_status launch_cache_write(hipStream_t s, bool bf16, const CacheMoveArgs &a);
 it_status launch_cache_read(hipStream_t s, bool bf16, const CacheMoveArgs &a);
@@ -115,9 +144,15 @@ struct GemmI8Args {
     int64_t M, N, K, lda, ldb, ldc;
     int out_bf16;
     int tiles_m, tiles_n;
+    const void *X;                  // launch_gemv_i8_x: the activations [M, xcols] in place of A and sA
+    int64_t ldx;
+    int xcols;
 };
 it_status launch_quantize_i8(hipStream_t s, bool bf16, int64_t rows, int64_t cols, const void *X, int64_t ldx,
                              int8_t *codes, int64_t ldc, float *steps);
 it_status launch_gemm_i8(it_context *ctx, GemmI8Args a);
+// Quantising and product in one launch, for few and short rows (K: the padded one).
+bool gemv_i8_x_applicable(int64_t M, int64_t K);
+it_status launch_gemv_i8_x(hipStream_t s, bool bf16, const GemmI8Args &a);
 
 }  // namespace it

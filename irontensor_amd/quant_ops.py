@@ -215,10 +215,10 @@ def cached_attention(q: Tensor, cache: KvCache, start: Union[Positions, Sequence
 
 class Int8Matrix:
     """A matrix [rows, cols] in 8-bit codes with an FP32 step for each row (quantize_i8): a weight with a step per
-    output channel, or activations with one per token. Rows are padded with zeros to a multiple of 16."""
+    output channel, or activations with one per token. Rows are padded with zeros to a multiple of 128."""
 
     def __init__(self, rows: int, cols: int, ctx: Context):
-        self.rows, self.cols, self.ld = int(rows), int(cols), (int(cols) + 15) // 16 * 16
+        self.rows, self.cols, self.ld = int(rows), int(cols), (int(cols) + 127) // 128 * 128
         self.ctx = ctx
         self._codes = _Buffer(ctx, self.rows * self.ld)
         self.steps = Tensor.empty([self.rows], _P.FP32, ctx)

@@ -136,7 +136,9 @@ def test_empty_products(it):
 
 @pytest.mark.parametrize("prec", ["f32", "bf16"])
 @pytest.mark.parametrize("m,n,k,bias", [(1, 768, 256, False), (1, 5, 1, True), (4, 688, 300, True), (16, 256, 1237, False),
-                                        (31, 100, 77, True), (129, 513, 301, False), (1000, 701, 300, True)])
+                                        (31, 100, 77, True), (129, 513, 301, False), (1000, 701, 300, True),
+                                        (2, 33, 700, False), (3, 17, 129, True), (7, 50, 4096, True), (8, 19, 4096, False),
+                                        (9, 64, 3640, True), (16, 100, 2048, True), (1, 40, 20001, False)])
 def test_linear(it, prec, m, n, k, bias):
     rng = np.random.default_rng(k)
     x, w = _round(rng.standard_normal((m, k)), prec), (rng.standard_normal((n, k)) * 0.02).astype(np.float32)

@@ -115,7 +115,7 @@ def test_gemm_arguments():
     assert linear(dtype=1) == _lib.IT_ERR_PRECISION
     for kw in ({"k": -1}, {"ldx": 29}, {"ldw": 16}, {"ldy": 4}, {"w": 260}, {"m": -1}):
         assert linear(**kw) == _lib.IT_ERR_INVALID, kw
-    assert linear(k=131057, ldx=131057, ldw=131072) == _lib.IT_ERR_DIMS
+    assert linear(k=130945, ldx=131057, ldw=131072) == _lib.IT_ERR_DIMS
     for name in ("x", "w", "sw", "y"):
         assert linear(**{name: None}) == _lib.IT_ERR_NULL, name
 
