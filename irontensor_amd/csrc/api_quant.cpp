@@ -61,7 +61,6 @@ it_status profiled(it_context *ctx, K key, F launch) {
 }
 
 bool f32_or_bf16(it_dtype d) { return d == IT_F32 || d == IT_BF16; }
-int64_t esize(it_dtype d) { return d == IT_BF16 ? 2 : 4; }
 
 it_status bad_dtype(const char *op) {
     return fail(IT_ERR_PRECISION, std::string(op) + ": precision mismatch, expected FP32 or BF16");
@@ -106,7 +105,7 @@ it_status geometry(const char *op, const it_kv_cache *c, it::CacheGeom *g) {
 it_status head_layout(const char *op, const it_attn_layout *l, int64_t heads, int64_t rows, int64_t d,
                       it::HeadLayout *out) {
     if (!l) {
-        *out = it::HeadLayout{1, rows * d, 0, d};
+        *out = it::HeadLayout{heads * rows * d, rows * d, d};
         return IT_OK;
     }
     if (l->heads < 1 || l->row_stride < d || l->batch_stride < 0 || l->head_stride < 0 || l->row_stride > MAX_DIM ||
@@ -114,13 +113,12 @@ it_status head_layout(const char *op, const it_attn_layout *l, int64_t heads, in
         return fail(IT_ERR_INVALID, std::string(op) + ": bad layout strides");
     if (l->heads != heads && l->heads != 1)
         return fail(IT_ERR_SHAPE, std::string(op) + ": shape mismatch, the layout's heads must be 1 or " + i64(heads) + ", got " + i64(l->heads));
-    *out = it::HeadLayout{l->heads, l->batch_stride, l->head_stride, l->row_stride};
+    // One head a batch stride ([batch * heads, ..]): the same address with the strides of a sequence and a head.
+    *out = l->heads == heads ? it::HeadLayout{l->batch_stride, l->head_stride, l->row_stride}
+                             : it::HeadLayout{heads * l->batch_stride, l->batch_stride, l->row_stride};
     return IT_OK;
 }
 
-bool vec16(const void *p, const it::HeadLayout &l, int64_t e) {
-    return (uintptr_t)p % 16 == 0 && l.bs * e % 16 == 0 && l.hs * e % 16 == 0 && l.rs * e % 16 == 0;
-}
 
 }  // namespace
 
@@ -215,13 +213,10 @@ it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache
         a.O = O;
         a.start = start;
         a.count = count;
-        a.heads = heads;
         a.n = n;
         a.share = (int)(heads / a.c.kv_heads);
         a.rows = (int)(n * a.share);
         a.scale_log2 = scale * 1.4426950408889634f;
-        a.q_vec = vec16(Q, a.ql, esize(dtype));
-        a.o_vec = vec16(O, a.ol, esize(dtype));
         const int64_t floats = it::plan_cached_attention(a, dtype == IT_BF16, ctx->num_cus);
         if (a.c.batch * a.c.kv_heads > MAX_GRID / a.row_blocks / a.splits) return fail(IT_ERR_DIMS, std::string(op) + ": too many queries");
         const OnDevice dev(ctx);

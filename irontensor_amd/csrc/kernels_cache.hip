@@ -94,18 +94,17 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
     constexpr int ROW = D * BITS / 8;             // bytes of a token's codes
     constexpr int BIAS = BITS == 4 ? 8 : 128;
     constexpr float L = BITS == 4 ? 7.f : 127.f;
-    const int64_t item = (int64_t)blockIdx.x * CM_THREADS + threadIdx.x;
-    const int c = (int)(item % OCT);
-    const int64_t unit = item / OCT;
-    const int64_t total = p.c.batch * p.c.kv_heads * p.blocks;
-    const bool live = unit < total;  // the same for all lanes of a unit, which shuffles among themselves
-    const int64_t bh = live ? unit / p.blocks : 0, blk = live ? unit % p.blocks : 0;
-    const int64_t b = bh / p.c.kv_heads;
+    // Units (a block of a head of a sequence) of OCT threads; 32-bit divisions, the 64-bit ones take 1 us.
+    const uint32_t unit = blockIdx.x * (uint32_t)(CM_THREADS / OCT) + threadIdx.x / OCT;
+    const int c = threadIdx.x % OCT;
+    const bool live = unit < p.units;  // the same for all lanes of a unit, which shuffles among themselves
+    const uint32_t bh = live ? unit / (uint32_t)p.blocks : 0, blk = live ? unit % (uint32_t)p.blocks : 0;
+    const uint32_t b = bh / (uint32_t)p.c.kv_heads, h = bh % (uint32_t)p.c.kv_heads;
     const int64_t p0 = p.start[b];
     int64_t cnt = p.n;
     if (p.count) cnt = min(cnt, max((int64_t)p.count[b], (int64_t)0));
     const int64_t pb = ((p0 >> 2) + blk) * 4;
-    const T *Kp = (const T *)p.K + p.lay.at(bh) + 8 * c, *Vp = (const T *)p.V + p.lay.at(bh) + 8 * c;
+    const T *Kp = (const T *)p.K + p.lay.at(b, h) + 8 * c, *Vp = (const T *)p.V + p.lay.at(b, h) + 8 * c;
     char *region = p.c.data + bh * p.c.region;
     Raw8<T> kx[4], vx[4];
     bool ok[4];
@@ -188,13 +187,13 @@ __global__ __launch_bounds__(CM_THREADS) void cache_read(const CacheMoveArgs p) 
     constexpr int ROW = D * BITS / 8;
     constexpr int BIAS = BITS == 4 ? 8 : 128;
     constexpr int WORDS = BITS;
-    const int64_t item = (int64_t)blockIdx.x * CM_THREADS + threadIdx.x;
-    const int c = (int)(item % OCT);
-    const int64_t unit = item / OCT;
-    if (unit >= p.c.batch * p.c.kv_heads * p.blocks) return;
-    const int64_t bh = unit / p.blocks, pb = ((p.begin >> 2) + unit % p.blocks) * 4;
+    const uint32_t unit = blockIdx.x * (uint32_t)(CM_THREADS / OCT) + threadIdx.x / OCT;
+    const int c = threadIdx.x % OCT;
+    if (unit >= p.units) return;
+    const uint32_t bh = unit / (uint32_t)p.blocks, b = bh / (uint32_t)p.c.kv_heads, h = bh % (uint32_t)p.c.kv_heads;
+    const int64_t pb = ((p.begin >> 2) + unit % (uint32_t)p.blocks) * 4;
     const char *region = p.c.data + bh * p.c.region;
-    T *Ko = (T *)p.Ko + p.lay.at(bh) + 8 * c, *Vo = (T *)p.Vo + p.lay.at(bh) + 8 * c;
+    T *Ko = (T *)p.Ko + p.lay.at(b, h) + 8 * c, *Vo = (T *)p.Vo + p.lay.at(b, h) + 8 * c;
     const int s = c / 4, g = c % 4;
     uint32_t w[WORDS];
     const u32x4 *vd = (const u32x4 *)(region + p.c.v_off + (pb / 4) * (4 * ROW) + c * (4 * WORDS));
@@ -232,9 +231,10 @@ __global__ __launch_bounds__(CM_THREADS) void cache_read(const CacheMoveArgs p) 
 }
 
 template <bool WRITE, typename T, int BITS>
-it_status launch_move(hipStream_t s, const CacheMoveArgs &a) {
-    const int64_t items = a.c.batch * a.c.kv_heads * a.blocks * (a.c.head_dim / 8);
-    const dim3 grid((unsigned)((items + CM_THREADS - 1) / CM_THREADS)), block(CM_THREADS);
+it_status launch_move(hipStream_t s, CacheMoveArgs a) {
+    a.units = a.c.batch * a.c.kv_heads * a.blocks;  // below 2^31, checked by the caller
+    const int64_t per = CM_THREADS / (a.c.head_dim / 8);
+    const dim3 grid((unsigned)((a.units + per - 1) / per)), block(CM_THREADS);
     const int d = a.c.head_dim;
     if constexpr (WRITE) {
         if (d == 64) hipLaunchKernelGGL((cache_write<T, BITS, 64>), grid, block, 0, s, a);

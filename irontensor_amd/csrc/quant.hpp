@@ -98,10 +98,10 @@ struct CacheGeom {
     int bits, head_dim;
 };
 
-// Per-head addressing of a 16- or 32-bit operand: (bh / heads) * bs + (bh % heads) * hs + row * rs + d.
+// Element (sequence b, head h, row, d) of a 16- or 32-bit operand: b * bs + h * hs + row * rs + d.
 struct HeadLayout {
-    int64_t heads, bs, hs, rs;
-    __host__ __device__ int64_t at(int64_t bh) const { return (bh / heads) * bs + (bh % heads) * hs; }
+    int64_t bs, hs, rs;
+    __host__ __device__ int64_t at(int64_t b, int64_t h) const { return b * bs + h * hs; }
 };
 
 struct CacheMoveArgs {
@@ -112,6 +112,7 @@ struct CacheMoveArgs {
     const int32_t *start, *count;
     int64_t begin, n;
     int64_t blocks;         // 4-token blocks of a (sequence, head) that the call may touch
+    int64_t units;          // blocks of all of them
 };
 it_status launch_cache_write(hipStream_t s, bool bf16, const CacheMoveArgs &a);
 it_status launch_cache_read(hipStream_t s, bool bf16, const CacheMoveArgs &a);
@@ -122,16 +123,17 @@ struct CachedAttnArgs {
     void *O;
     HeadLayout ql, ol;
     const int32_t *start, *count;
-    int64_t heads, n;       // query heads; queries of a sequence
+    int64_t n;              // queries of a sequence
     int share;              // query heads of one cache head
     int rows;               // n * share
+    int row_tiles;          // 16-row tiles of a block
     int row_blocks, splits;
+    float per_key;          // keys of a block for each key of the batch, to spread them evenly
     float scale_log2;       // scale * log2 e
     float *part;            // splits > 1: partial results, and
     int *counters;          // one arrival counter for each (sequence, head, row block)
-    int q_vec, o_vec;
 };
-// Fills in row_blocks and splits; the floats of `part` that the launch then needs (0: none).
+// Fills in row_tiles, row_blocks, splits and per_key; the floats of `part` that the launch then needs (0: none).
 int64_t plan_cached_attention(CachedAttnArgs &a, bool bf16, int num_cus);
 it_status launch_cached_attention(hipStream_t s, bool bf16, const CachedAttnArgs &a);
 
