@@ -513,8 +513,8 @@ it_status it_lion_step(it_context *ctx, int count, float *const *weights, float 
  * current one is, allocate nothing but library scratch (grown once per shape, not during a capture), and
  * are deterministic.
  *
- * Quantising a group of values: step s = max|x| / L with L = 7 (4 bits) or 127 (8 bits), codes = x / s
- * rounded to nearest even (the real quotient's rounding), value = code * s. A step below 2^-126 is 0 and
+ * Quantising a group of values: step s = max|x| * (1 / L), in FP32 with 1 / L rounded, L = 7 (4 bits) or 127
+ * (8 bits); codes = x / s rounded to nearest even (the real quotient's rounding); value = code * s. A step below 2^-126 is 0 and
  * the group reads as zeros; a group that holds a NaN or an infinity reads as NaN.
  */
 

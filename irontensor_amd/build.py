@@ -28,7 +28,7 @@ SOURCES = ["runtime.cpp", "api.cpp", "api_train.cpp", "kernels_gemm.hip", "kerne
            "kernels_flash.hip", "kernels_gemv.hip", "kernels_train.hip", "noalloc.hip", "kernels_flash2.hip",
            "api_quant.cpp", "kernels_cache.hip", "kernels_cached_attn.hip", "kernels_i8.hip"]
 #: Sources with planner overrides (IT_TUNING).
-TUNED = ["kernels_gemm.hip", "kernels_gemm_f32.hip", "kernels_i8.hip", "kernels_cached_attn.hip"]
+TUNED = ["kernels_gemm.hip", "kernels_gemm_f32.hip"]
 
 # -packed-fp32-ops: hipcc must not emit packed FP32 ALU ops (v_pk_*_f32) on this pool.
 HIP_FLAGS = [

@@ -27,7 +27,6 @@
 //     (m, l, O) are joined by the waves through LDS and by the row block's last block to arrive.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "quant.hpp"
 
@@ -41,7 +40,7 @@ constexpr int CA_DEVICE_SCOPE = 16;    // cache-policy bit sc1 of the buffer int
 constexpr int64_t CA_MIN_CHUNK = 256;  // keys of a split, at least
 constexpr int CA_MAX_SPLITS = 128;
 constexpr int CA_JOIN = 16;            // partial results a thread loads at a time in the join
-constexpr int CA_TARGET = 4;           // blocks a CU that the splits aim at
+constexpr int CA_TARGET = 1;           // blocks a CU that the splits aim at
 // Blocks that a CU holds, by registers and by their rings of LDS: four with one row tile of up to 128 BF16
 // channels (three in FP32), two otherwise.
 constexpr int ca_blocks(bool f32, int d, int rt) { return rt == 1 && d <= 128 ? (f32 ? 3 : 4) : 2; }
@@ -124,29 +123,30 @@ struct CachedAttn {
     static constexpr int NB = FIT > 6 ? 6 : FIT < 2 ? 2 : FIT;
     static_assert(CODES % 1024 == 0 && NB * LOADS < 64, "whole loads, counted by vmcnt");
 
-    // Tokens t .. t + 31 (t a multiple of 32) into `slot`; an invalid tile loads nothing (zeros), and so do lanes
-    // past the region's end (the range check goes by the vector offset).
+    // Tokens t .. t + 31 (t a multiple of 32) into `slot`; an invalid tile loads nothing (zeros). A descriptor of
+    // exactly the 32 tokens for each of the four arrays: scalar arithmetic, and a lane's offset never changes.
     __device__ __forceinline__ static void issue(const CacheGeom &c, const char *region, uint32_t t, bool valid, uint32_t slot,
                                                  int lane) {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<char *>(region), (short)0, valid ? (int)c.region : 0, 0x00020000);
-        auto load16 = [&](uint32_t to, uint32_t from) {
+        auto array = [&](int64_t at, int bytes) {
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(region + at), (short)0, valid ? bytes : 0, 0x00020000);
+        };
+        auto to_lds = [&](uint32_t to) {
             uint32_t x = slot + to;
             asm("" : "+s"(x));  // opaque: the waits in the loop order these loads
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (ca_lds_t *)(uintptr_t)x, 16, from + 16 * lane, 0, 0, 0);
+            return (ca_lds_t *)(uintptr_t)x;
         };
-        auto load4 = [&](uint32_t to, uint32_t from) {
-            uint32_t x = slot + to;
-            asm("" : "+s"(x));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (ca_lds_t *)(uintptr_t)x, 4, from + 4 * lane, 0, 0, 0);
-        };
+        const __amdgpu_buffer_rsrc_t k = array((int64_t)t * ROW, CODES), v = array(c.v_off + (int64_t)t * ROW, CODES);
 #pragma unroll
-        for (int i = 0; i < CODES / 1024; ++i) load16(1024 * i, t * ROW + 1024 * i);
+        for (int i = 0; i < CODES / 1024; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(k, to_lds(1024 * i), 16, 16 * lane + 1024 * i, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < CODES / 1024; ++i) load16(CODES + 1024 * i, (uint32_t)c.v_off + t * ROW + 1024 * i);
+        for (int i = 0; i < CODES / 1024; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(v, to_lds(CODES + 1024 * i), 16, 16 * lane + 1024 * i, 0, 0, 0);
+        const __amdgpu_buffer_rsrc_t ks = array(c.ks_off + (int64_t)t * (2 * G), CA_TT * 2 * G), vs = array(c.vs_off + (int64_t)t * 2, CA_TT * 2);
 #pragma unroll
-        for (int i = 0; i < KS_LOADS; ++i) load4(KS_AT + 256 * i, (uint32_t)c.ks_off + t * (2 * G) + 256 * i);
-        load4(VS_AT, (uint32_t)c.vs_off + t * 2);  // 64 bytes; the rest is not used
+        for (int i = 0; i < KS_LOADS; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, to_lds(KS_AT + 256 * i), 4, 4 * lane + 256 * i, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, to_lds(VS_AT), 4, 4 * lane, 0, 0, 0);
     }
 
     // Codes and steps of 16 tokens' keys (half h of a slot); the steps of token 4 g + r, group s at word
@@ -228,12 +228,15 @@ void cached_attn(const CachedAttnArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
 
-    // The block's place: row block fastest, so that blocks that share keys are near each other, and a
-    // contiguous range of places on every XCD (workgroup w runs on XCD w % 8).
+    // The block's place: row block fastest, split slowest. Splits that a sequence has no keys for end at once, and
+    // in this order they are the last to be dispatched: between the others they left CUs empty beside CUs
+    // with two blocks (131072 tokens of 8 heads: 51.7 us against 40). Row blocks share keys, so where there are
+    // several every XCD (workgroup w runs on XCD w % 8) takes a contiguous range of places.
     uint32_t pid = blockIdx.x;
-    if (gridDim.x % 8 == 0) pid = (pid % 8) * (gridDim.x / 8) + pid / 8;
-    const uint32_t rest = pid / (uint32_t)p.row_blocks, unit = rest / (uint32_t)p.splits;  // sequence * kv_heads + cache head
-    const int rb = (int)(pid % (uint32_t)p.row_blocks), split = (int)(rest % (uint32_t)p.splits);
+    if (p.row_blocks > 1 && gridDim.x % 8 == 0) pid = (pid % 8) * (gridDim.x / 8) + pid / 8;
+    const uint32_t units = (uint32_t)(p.c.batch * p.c.kv_heads), rest = pid / (uint32_t)p.row_blocks;
+    const int rb = (int)(pid % (uint32_t)p.row_blocks), split = (int)(rest / units);
+    const uint32_t unit = rest % units;  // sequence * kv_heads + cache head
     const uint32_t b = unit / (uint32_t)p.c.kv_heads, kvh = unit % (uint32_t)p.c.kv_heads;
     const char *region = p.c.data + unit * p.c.region;
     const int row0 = rb * ROWS;
@@ -299,7 +302,7 @@ void cached_attn(const CachedAttnArgs p) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = 0.f;
-                if (lim[rt] > 0) {
+                if (row < p.rows) {
                     const f32x4 lo = *(const f32x4_any *)(src + 32 * s), hi = *(const f32x4_any *)(src + 32 * s + 4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
@@ -313,7 +316,7 @@ void cached_attn(const CachedAttnArgs p) {
                 }
             } else {
                 u32x4 x = {0u, 0u, 0u, 0u};
-                if (lim[rt] > 0) x = *(const u32x4_any *)(src + 32 * s);
+                if (row < p.rows) x = *(const u32x4_any *)(src + 32 * s);
                 q[rt][s][0] = x;
                 float sum = 0.f;
 #pragma unroll
@@ -631,16 +634,13 @@ int64_t plan_cached_attention(CachedAttnArgs &a, bool bf16, int num_cus) {
     const int rows = 16 * a.row_tiles;
     a.row_blocks = (a.rows + rows - 1) / rows;
     const int64_t units = a.c.batch * a.c.kv_heads * a.row_blocks;
-    // Splits that leave a block CA_MIN_CHUNK keys at least, and twice the blocks aimed at in the grid, so that a
-    // ragged batch's long sequences can take more than their even part.
-    int64_t target = CA_TARGET * num_cus, most = CA_MAX_SPLITS;
-#ifdef IT_TUNING
-    if (const char *e = getenv("IT_CA_TARGET")) target = atoi(e) * num_cus;
-    if (const char *e = getenv("IT_CA_SPLITS")) most = atoi(e);
-#endif
+    // Splits for one block a CU, of CA_MIN_CHUNK keys at least, and twice as many in the grid, so that a ragged
+    // batch's long sequences can take more than their even part. More blocks stream no faster and their joins
+    // cost more: 32768 tokens of 8 heads take 19.6 us with one block a CU, 22.6 with two, 33 with four.
+    const int64_t target = CA_TARGET * num_cus;
     a.per_key = (float)((double)(a.c.kv_heads * a.row_blocks) / (double)target);
     int64_t splits = 2 * target / units;
-    splits = std::min({splits, (a.c.capacity + CA_MIN_CHUNK - 1) / CA_MIN_CHUNK, most});
+    splits = std::min({splits, (a.c.capacity + CA_MIN_CHUNK - 1) / CA_MIN_CHUNK, (int64_t)CA_MAX_SPLITS});
     if (units > COUNTERS || splits < 2) splits = 1;
     a.splits = (int)splits;
     return splits > 1 ? units * splits * rows * (a.c.head_dim + 4) : 0;

@@ -9,7 +9,8 @@ namespace it {
 
 // ------------------------------------------------------------------ the quantiser
 
-// A group of values shares the step s = max|x| / L (L: the largest code) and keeps n = rne(x / s). A step
+// A group of values shares the step s = max|x| * (1 / L) (L: the largest code; FP32, 1 / L rounded) and keeps
+// n = rne(x / s) of the step as it is stored. A step
 // below the smallest normal number is stored as 0 (the group reads as zeros); a group that holds a NaN or
 // an infinity gets s = NaN and codes 0, so that all of it reads as NaN.
 constexpr float QUANT_TINY = 1.17549435e-38f;  // 2^-126
@@ -21,7 +22,7 @@ constexpr float QUANT_TINY = 1.17549435e-38f;  // 2^-126
 template <bool BF16>
 __device__ __forceinline__ float quant_step(uint32_t maxbits, float levels) {
     if (maxbits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    float s = __uint_as_float(maxbits) / levels;
+    float s = __uint_as_float(maxbits) * (1.f / levels);
     if constexpr (BF16) s = bf16_to_f32(f32_to_bf16_rne(s));
     return s < QUANT_TINY ? 0.f : s;
 }
@@ -35,7 +36,7 @@ __device__ __forceinline__ float quant_inverse(float s) { return s > 0.f ? 1.f /
 // is its comparison with s / 2: above it the code is the next one, at it the even one. That repair is a
 // branch that FP32 values hardly ever take and BF16 ones, which hit halves exactly, in every third pair of a
 // wave. A quotient never passes the largest code L by a half: s is within 2^-8 (BF16) of max|x| / L, and
-// 127 / (1 - 2^-8) < 127.5.
+// 127 / (1 - 2^-8) (1 + 2^-22) < 127.5.
 template <int BIAS>
 __device__ __forceinline__ void quant_codes(const float (&x)[8], float s, float inv, uint32_t (&u)[8]) {
     constexpr float MAGIC = 12582912.f + BIAS;  // 3 2^22 + BIAS

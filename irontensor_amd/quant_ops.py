@@ -240,7 +240,7 @@ class Int8Matrix:
 
 
 def quantize_i8(x: Tensor) -> Int8Matrix:
-    """x [rows, cols] (FP32 or BF16) as 8-bit codes with a step per row, max|row| / 127."""
+    """x [rows, cols] (FP32 or BF16) as 8-bit codes with a step per row, max|row| * (1 / 127)."""
     op = "quantize_i8"
     if len(x.shape()) != 2:
         raise UnsupportedDimensions(op, "a 2D tensor", x.shape())

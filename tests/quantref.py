@@ -14,11 +14,11 @@ def rne_bf16(x):
 
 
 def steps(x, group, levels, bf16=True):
-    """[.., D / group] FP32 steps of x [.., D]: max|x| / levels, NaN where a value is not finite."""
+    """[.., D / group] FP32 steps of x [.., D]: max|x| * (1 / levels), NaN where a value is not finite."""
     g = np.asarray(x, np.float32).reshape(*x.shape[:-1], x.shape[-1] // group, group)
     with np.errstate(invalid="ignore"):
         most = np.abs(g).max(-1)
-    s = most / np.float32(levels)
+        s = most * (np.float32(1) / np.float32(levels))
     if bf16:
         s = rne_bf16(s)
     s = np.where(s < TINY, np.float32(0), s)
