@@ -848,4 +848,180 @@ inline FusedLinearCE fused_linear_cross_entropy(const Tensor &hidden, const Tens
     return r;
 }
 
+// ------------------------------------------------------------------ quantised serving
+// A key/value cache in 4 or 8 bits, the attention that reads it and the linear layer on an 8-bit weight. No
+// counterpart in the reference, whose inference recomputes the whole prompt for every token (src/inference).
+
+// int32 words on the device, one for each sequence (raw words in a [n] FP32-sized tensor).
+inline Tensor upload_positions(const std::vector<int32_t> &values) {
+    Tensor t = Tensor::empty({values.size()}, Precision::FP32);
+    if (!values.empty())
+        check(it_memcpy_h2d(Context::global().handle(), t.data(), values.data(), values.size() * 4), "upload_positions");
+    return t;
+}
+
+// Keys and values of up to `capacity` tokens of `batch` sequences with `kv_heads` heads of 64, 128 or 256 channels;
+// starts as zeros.
+class KvCache {
+  public:
+    KvCache(size_t batch, size_t kv_heads, size_t capacity, size_t head_dim, int bits = 4)
+        : desc_{bits, (int64_t)batch, (int64_t)kv_heads, (int64_t)capacity, (int64_t)head_dim, nullptr},
+          bytes_(size_of(desc_)), data_(Tensor::zeros({(bytes_ + 3) / 4}, Precision::FP32)) {
+        desc_.data = data_.data();
+    }
+    const it_kv_cache &desc() const { return desc_; }
+    size_t bytes() const { return bytes_; }
+    size_t batch() const { return (size_t)desc_.batch; }
+    size_t kv_heads() const { return (size_t)desc_.kv_heads; }
+    size_t head_dim() const { return (size_t)desc_.head_dim; }
+    void clear() {
+        if (bytes_) check(it_zero(Context::global().handle(), data_.data(), bytes_), "kv_cache");
+    }
+
+  private:
+    static size_t size_of(const it_kv_cache &d) {
+        size_t n = 0;
+        check(it_kv_cache_bytes(d.bits, d.batch, d.kv_heads, d.capacity, d.head_dim, &n), "kv_cache");
+        return n;
+    }
+    it_kv_cache desc_;
+    size_t bytes_;
+    Tensor data_;
+};
+
+namespace detail {
+inline it_attn_layout bshd(size_t seq, size_t heads, size_t dim) {
+    const int64_t h = heads ? (int64_t)heads : 1, d = (int64_t)dim;
+    return it_attn_layout{h, (int64_t)seq * h * d, d, h * d};
+}
+inline const int32_t *positions(const char *op, const Tensor *t, size_t batch) {
+    if (!t) return nullptr;
+    if (t->numel() != batch || !t->is_f32()) throw ShapeMismatch(op, std::to_string(batch) + " positions", shape_str(t->shape()));
+    return (const int32_t *)t->data();
+}
+inline void need_4d(const char *op, const Tensor &t) {
+    if (t.shape().size() != 4) throw UnsupportedDimensions(op, "4D tensor [batch, seq, heads, dim]", t.shape());
+    if (!t.is_f32() && !t.is_bf16()) throw PrecisionMismatch(op, "FP32 or BF16", precision_name(t.precision()));
+}
+inline void same(const char *op, const Tensor &a, const Tensor &b) {
+    if (a.shape() != b.shape()) throw ShapeMismatch(op, shape_str(a.shape()), shape_str(b.shape()));
+    if (a.precision() != b.precision()) throw PrecisionMismatch(op, precision_name(a.precision()), precision_name(b.precision()));
+}
+}  // namespace detail
+
+// k, v [batch, n, kv_heads, head_dim] into positions start[b] .. of the cache (count: the first count[b] tokens).
+inline void kv_cache_write(const KvCache &cache, const Tensor &k, const Tensor &v, const Tensor &start,
+                           const Tensor *count = nullptr) {
+    const char *op = "kv_cache_write";
+    detail::need_4d(op, k);
+    detail::same(op, k, v);
+    const size_t n = k.shape()[1];
+    const std::vector<size_t> want{cache.batch(), n, cache.kv_heads(), cache.head_dim()};
+    if (k.shape() != want) throw ShapeMismatch(op, shape_str(want), shape_str(k.shape()));
+    const it_attn_layout lay = detail::bshd(n, cache.kv_heads(), cache.head_dim());
+    check(it_kv_cache_write(Context::global().handle(), (it_dtype)k.precision(), &cache.desc(), (int64_t)n, &lay, k.data(),
+                            v.data(), detail::positions(op, &start, cache.batch()),
+                            detail::positions(op, count, cache.batch())),
+          op);
+}
+
+// (K, V) [batch, n, kv_heads, head_dim] that positions begin .. begin + n - 1 stand for.
+inline std::pair<Tensor, Tensor> kv_cache_read(const KvCache &cache, size_t begin, size_t n,
+                                               Precision precision = Precision::FP32) {
+    const std::vector<size_t> shape{cache.batch(), n, cache.kv_heads(), cache.head_dim()};
+    std::pair<Tensor, Tensor> kv{Tensor::empty(shape, precision), Tensor::empty(shape, precision)};
+    const it_attn_layout lay = detail::bshd(n, cache.kv_heads(), cache.head_dim());
+    check(it_kv_cache_read(Context::global().handle(), (it_dtype)precision, &cache.desc(), (int64_t)begin, (int64_t)n, &lay,
+                           kv.first.data(), kv.second.data()),
+          "kv_cache_read");
+    return kv;
+}
+
+// softmax(scale Q.K^T).V of q [batch, n, heads, head_dim] over the cache: query i of sequence b sees the positions up to
+// start[b] + i. scale 0: 1 / sqrt(head_dim).
+inline Tensor cached_attention(const Tensor &q, const KvCache &cache, const Tensor &start, const Tensor *count = nullptr,
+                               float scale = 0.f) {
+    const char *op = "cached_attention";
+    detail::need_4d(op, q);
+    const size_t n = q.shape()[1], h = q.shape()[2], d = q.shape()[3];
+    if (q.shape()[0] != cache.batch() || d != cache.head_dim())
+        throw ShapeMismatch(op, shape_str({cache.batch(), n, h, cache.head_dim()}), shape_str(q.shape()));
+    Tensor out = Tensor::empty(q.shape(), q.precision());
+    const it_attn_layout lay = detail::bshd(n, h, d);
+    check(it_cached_attention(Context::global().handle(), (it_dtype)q.precision(), &cache.desc(), (int64_t)h, (int64_t)n,
+                              scale == 0.f ? 1.f / std::sqrt((float)d) : scale, &lay, nullptr, q.data(),
+                              detail::positions(op, &start, cache.batch()), detail::positions(op, count, cache.batch()),
+                              out.data()),
+          op);
+    return out;
+}
+
+// A matrix [rows, cols] in 8-bit codes with an FP32 step for each row; rows padded with zeros to a multiple of 128.
+class Int8Matrix {
+  public:
+    Int8Matrix(size_t rows, size_t cols)
+        : rows_(rows), cols_(cols), ld_((cols + 127) / 128 * 128), codes_(Tensor::empty({rows, ld_ / 4}, Precision::FP32)),
+          steps_(Tensor::empty({rows}, Precision::FP32)) {}
+    size_t rows() const { return rows_; }
+    size_t cols() const { return cols_; }
+    size_t ld() const { return ld_; }
+    int8_t *codes() const { return (int8_t *)codes_.data(); }
+    const Tensor &steps() const { return steps_; }
+
+  private:
+    size_t rows_, cols_, ld_;
+    Tensor codes_, steps_;
+};
+
+inline Int8Matrix quantize_i8(const Tensor &x) {
+    const char *op = "quantize_i8";
+    if (x.shape().size() != 2) throw UnsupportedDimensions(op, "2D tensor", x.shape());
+    Int8Matrix m(x.shape()[0], x.shape()[1]);
+    check(it_quantize_i8(Context::global().handle(), (it_dtype)x.precision(), (int64_t)m.rows(), (int64_t)m.cols(), x.data(),
+                         (int64_t)m.cols(), m.codes(), (int64_t)m.ld(), (float *)m.steps().data()),
+          op);
+    return m;
+}
+
+namespace detail {
+inline const float *bias_of(const char *op, const Tensor *bias, size_t n) {
+    if (!bias) return nullptr;
+    if (!bias->is_f32()) throw PrecisionMismatch(op, "FP32 bias", precision_name(bias->precision()));
+    if (bias->numel() != n) throw ShapeMismatch(op, "bias of " + std::to_string(n) + " elements", shape_str(bias->shape()));
+    return (const float *)bias->data();
+}
+}  // namespace detail
+
+// a.b^T of the values the two stand for, plus an FP32 bias.
+inline Tensor matmul_i8(const Int8Matrix &a, const Int8Matrix &b, const Tensor *bias = nullptr,
+                        Precision out_precision = Precision::FP32) {
+    const char *op = "matmul_i8";
+    if (a.cols() != b.cols()) throw InnerDimensionMismatch(op, {a.rows(), a.cols()}, {b.rows(), b.cols()});
+    const float *bp = detail::bias_of(op, bias, b.rows());
+    Tensor out = Tensor::empty({a.rows(), b.rows()}, out_precision);
+    check(it_gemm_i8(Context::global().handle(), (it_dtype)out_precision, (int64_t)a.rows(), (int64_t)b.rows(),
+                     (int64_t)a.ld(), a.codes(), (int64_t)a.ld(), (const float *)a.steps().data(), b.codes(), (int64_t)b.ld(),
+                     (const float *)b.steps().data(), bp, out.data(), (int64_t)b.rows()),
+          op);
+    return out;
+}
+
+// nn::Linear::forward (src/nn/linear.rs:87-145) on an 8-bit weight: x [.., in] quantised per token.
+inline Tensor linear_i8(const Tensor &x, const Int8Matrix &weight, const Tensor *bias = nullptr) {
+    const char *op = "linear_i8";
+    detail::require(!x.shape().empty(), "Input must have at least one dimension");
+    if (x.shape().back() != weight.cols()) throw InnerDimensionMismatch(op, x.shape(), {weight.rows(), weight.cols()});
+    const float *bp = detail::bias_of(op, bias, weight.rows());
+    std::vector<size_t> shape = x.shape();
+    shape.back() = weight.rows();
+    size_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+    Tensor out = Tensor::empty(shape, x.precision());
+    check(it_linear_i8(Context::global().handle(), (it_dtype)x.precision(), (int64_t)rows, (int64_t)weight.rows(),
+                       (int64_t)weight.cols(), x.data(), (int64_t)weight.cols(), weight.codes(), (int64_t)weight.ld(),
+                       (const float *)weight.steps().data(), bp, out.data(), (int64_t)weight.rows()),
+          op);
+    return out;
+}
+
 }  // namespace irontensor

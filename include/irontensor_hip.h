@@ -559,7 +559,10 @@ it_status it_kv_cache_read(it_context *ctx, it_dtype dtype, const it_kv_cache *c
  * [batch, heads, n, head_dim] contiguous or through q_layout and o_layout (NULL: q_layout), strides and
  * alignment as they come (16-byte multiples are faster). scale finite and > 0. FP32 results carry FP32
  * accuracy for the values the cache stands for; with BF16, probabilities are rounded to BF16 before their
- * product with the values. */
+ * product with the values. Sums run before their division by the row's sum: |v| times the positions seen
+ * has to stay below 2^117. Few queries over many positions are split among blocks, with partial results in
+ * scratch; where the scratch cannot be had (a capture that no eager call of the size came before) they are
+ * not, which takes longer and rounds differently. */
 it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache *cache, int64_t heads, int64_t n,
                               float scale, const it_attn_layout *q_layout, const it_attn_layout *o_layout,
                               const void *Q, const int32_t *start, const int32_t *count, void *O);

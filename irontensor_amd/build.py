@@ -97,17 +97,20 @@ def build_tuning_library() -> Path:
 
 CPP_TEST_SRC = ROOT / "tests" / "cpp" / "test_host_api.cpp"
 CPP_TEST_BIN = ROOT / "tests" / "cpp" / "_build" / "test_host_api"
+QUANT_TEST_SRC = ROOT / "tests" / "cpp" / "test_quant_api.cpp"
+QUANT_TEST_BIN = ROOT / "tests" / "cpp" / "_build" / "test_quant_api"
 
 
 def build_cpp_tests() -> Path:
-    """Builds the C++ host-API test program against the in-tree library (rpath-relative)."""
+    """Builds the C++ host-API test programs against the in-tree library (rpath-relative)."""
     CPP_TEST_BIN.parent.mkdir(parents=True, exist_ok=True)
-    cmd = ["g++", "-std=c++17", "-O1", "-Wall", f"-I{ROOT / 'include'}", str(CPP_TEST_SRC),
-           "-o", str(CPP_TEST_BIN), f"-L{PKG}", "-lirontensor_hip",
-           "-Wl,-rpath,$ORIGIN/../../../irontensor_amd", "-Wl,-rpath,/opt/rocm/lib"]
-    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"C++ host API test build failed:\n{res.stdout}")
+    for src, exe in ((CPP_TEST_SRC, CPP_TEST_BIN), (QUANT_TEST_SRC, QUANT_TEST_BIN)):
+        cmd = ["g++", "-std=c++17", "-O1", "-Wall", f"-I{ROOT / 'include'}", str(src),
+               "-o", str(exe), f"-L{PKG}", "-lirontensor_hip",
+               "-Wl,-rpath,$ORIGIN/../../../irontensor_amd", "-Wl,-rpath,/opt/rocm/lib"]
+        res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"C++ host API test build failed:\n{res.stdout}")
     return CPP_TEST_BIN
 
 

@@ -203,7 +203,7 @@ it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache
         if (!(scale > 0.f) || !std::isfinite(scale)) return fail(IT_ERR_INVALID, std::string(op) + ": scale must be finite and positive");
         if (heads > 0 && (a.c.kv_heads == 0 || heads % a.c.kv_heads != 0))
             return fail(IT_ERR_SHAPE, std::string(op) + ": shape mismatch, expected heads divisible by the cache's " + i64(a.c.kv_heads) + ", got " + i64(heads));
-        if (heads > MAX_GRID || (heads > 0 && n > MAX_GRID / heads)) return fail(IT_ERR_DIMS, std::string(op) + ": too many queries");
+        if (heads > MAX_GRID / 2 || (heads > 0 && n > MAX_GRID / 2 / heads)) return fail(IT_ERR_DIMS, std::string(op) + ": too many queries");
         if (const it_status st = head_layout(op, q_layout, heads, n, a.c.head_dim, &a.ql); st != IT_OK) return st;
         if (const it_status st = head_layout(op, o_layout, heads, n, a.c.head_dim, &a.ol); st != IT_OK) return st;
         if (!o_layout) a.ol = a.ql;
@@ -221,10 +221,14 @@ it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache
         if (a.c.batch * a.c.kv_heads > MAX_GRID / a.row_blocks / a.splits) return fail(IT_ERR_DIMS, std::string(op) + ": too many queries");
         const OnDevice dev(ctx);
         if (floats > 0) {
+            // Without scratch (a capture before any eager call, no memory) every row block takes all its keys.
             void *part = nullptr;
-            if (const it_status st = it::ensure_scratch(ctx, (size_t)floats * sizeof(float), &part); st != IT_OK) return st;
-            if (const it_status st = it::ensure_counters(ctx, &a.counters); st != IT_OK) return st;
-            a.part = (float *)part;
+            if (it::ensure_scratch(ctx, (size_t)floats * sizeof(float), &part) == IT_OK && it::ensure_counters(ctx, &a.counters) == IT_OK) {
+                a.part = (float *)part;
+            } else {
+                it::clear_error();
+                a.splits = 1;
+            }
         }
         return profiled(
             ctx, [&] { return "cached_attn" + i64(a.c.bits) + "[" + i64(a.c.batch) + "x" + i64(heads) + "/" + i64(a.c.kv_heads) + "x" + i64(n) + "x" + i64(a.c.head_dim) + ",T=" + i64(a.c.capacity) + "]"; },

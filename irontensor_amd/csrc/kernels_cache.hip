@@ -9,6 +9,7 @@
 #include <algorithm>
 
 #include "quant.hpp"
+#include "quantiser.hpp"
 
 namespace it {
 namespace {

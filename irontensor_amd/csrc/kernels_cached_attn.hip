@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "mfma.hpp"
 #include "quant.hpp"
 
 namespace it {

@@ -13,6 +13,7 @@
 
 #include "gemm_tiles.hpp"
 #include "quant.hpp"
+#include "quantiser.hpp"
 
 namespace it {
 namespace {

@@ -266,6 +266,23 @@ def test_hidden_positions_do_not_matter(it, prec, bits, n):
 
 
 @pytest.mark.parametrize("prec", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [4, 70])
+def test_padded_queries_do_not_matter(it, prec, n):
+    """Queries at count and beyond may hold anything: zeros come out, and the others' bits stay."""
+    b, hkv, share, d, cap = 2, 2, 3, 64, 90
+    rng = np.random.default_rng(n)
+    k, v = (_tensor(it, _keys(rng, (b, cap, hkv, d), prec), prec) for _ in range(2))
+    cache = it.KvCache(b, hkv, cap, d, 4)
+    it.kv_cache_write(cache, k, v, [0] * b)
+    q = _round(rng.standard_normal((b, n, hkv * share, d)), prec)
+    start, count = it.upload_positions([5, 0]), it.upload_positions([n - 3, 1])
+    clean = it.cached_attention(_tensor(it, q, prec), cache, start, count).numpy()
+    q[0, n - 3:], q[1, 1:] = np.nan, np.inf
+    got = it.cached_attention(_tensor(it, q, prec), cache, start, count).numpy()
+    assert np.array_equal(got, clean) and not got[0, n - 3:].any() and not got[1, 1:].any() and got[0, 0].any()
+
+
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
 def test_visible_nan_and_infinity(it, prec):
     for which in ("k", "v"):
         def fill(k, v):

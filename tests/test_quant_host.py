@@ -1,0 +1,91 @@
+"""The quantised serving operators' host side on the CPU, with the stand-in HIP runtime of test_host_dispatch.py:
+which kernels a call launches, and what it does when scratch cannot be had."""
+from __future__ import annotations
+
+from test_host_dispatch import _run, fake  # noqa: F401  (the fixture)
+
+CALLS = """
+import numpy as np
+def attend(cache, n, heads, start):
+    q = it.Tensor.empty([cache.batch, n, heads, cache.head_dim], it.Precision.BF16)
+    launches()
+    it.cached_attention(q, cache, start, out=q)
+    return launches()
+def linear(m, n, k):
+    w = it.quantize_i8(it.Tensor.empty([n, k]))
+    x = it.Tensor.empty([m, k])
+    launches()
+    it.linear_i8(x, w)
+    return launches()
+"""
+
+
+def test_launches(fake):  # noqa: F811
+    """One launch each for a write, a read, attention (split or not) and a small layer; two for a larger layer."""
+    _run(fake, CALLS + """
+cache = it.KvCache(1, 2, 5000, 64, 4)
+pos = it.upload_positions([7])
+kv = it.Tensor.empty([1, 3, 2, 64])
+launches()
+it.kv_cache_write(cache, kv, kv, pos)
+it.kv_cache_read(cache, 4, 9)
+got = launches()
+assert len(got) == 2 and "cache_write" in got[0] and "cache_read" in got[1], got
+for n, heads in ((1, 2), (1, 32), (5, 6), (300, 4)):
+    got = attend(cache, n, heads, pos)
+    assert len(got) == 1 and "cached_attn" in got[0], got
+assert ["gemv_i8_x" in x for x in linear(1, 40, 200)] == [True]
+got = linear(16, 40, 2000)
+assert len(got) == 2 and "quantize_rows" in got[0] and "gemv_i8" in got[1], got
+got = linear(17, 40, 200)
+assert len(got) == 2 and "quantize_rows" in got[0] and "gemm_i8_tile" in got[1], got
+assert linear(0, 40, 200) == [] and attend(cache, 0, 4, pos) == []
+""")
+
+
+def test_refused_scratch(fake):  # noqa: F811
+    """Attention runs unsplit where its scratch is refused; a layer that needs scratch says so and launches nothing."""
+    _run(fake, CALLS + """
+cache = it.KvCache(1, 2, 5000, 64, 4)
+pos = it.upload_positions([7])
+x, w = it.Tensor.empty([40, 300]), it.quantize_i8(it.Tensor.empty([50, 300]))
+y, q = it.Tensor.empty([40, 50]), it.Tensor.empty([1, 1, 2, 64])
+launches()
+fake.fake_hip_limit(1 << 20)
+it.cached_attention(q, cache, pos, out=q)
+got = launches()
+assert len(got) == 1 and "cached_attn" in got[0], got
+assert ctx.lib.it_mem_scratch(ctx.handle) == 0
+try:
+    it.linear_i8(x, w, out=y)
+    raise SystemExit("not refused")
+except it.DeviceError as e:
+    assert "out of device memory" in str(e)
+assert launches() == []
+fake.fake_hip_limit((1 << 64) - 1)
+it.linear_i8(x, w, out=y)
+it.cached_attention(q, cache, pos, out=q)
+assert len(launches()) == 3 and ctx.lib.it_mem_scratch(ctx.handle) > 0
+""")
+
+
+def test_capture_without_scratch(fake):  # noqa: F811
+    """A capture before any eager call records attention unsplit and refuses a layer that needs scratch."""
+    _run(fake, CALLS + """
+cache = it.KvCache(1, 2, 5000, 64, 4)
+pos = it.upload_positions([7])
+x, w = it.Tensor.empty([40, 300]), it.quantize_i8(it.Tensor.empty([50, 300]))
+y, q = it.Tensor.empty([40, 50]), it.Tensor.empty([1, 1, 2, 64])
+launches()
+assert ctx.lib.it_capture_begin(ctx.handle) == 0
+it.cached_attention(q, cache, pos, out=q)
+try:
+    it.linear_i8(x, w, out=y)
+    raise SystemExit("not refused")
+except it.InvalidValue as e:
+    assert "run the work once before capturing" in str(e)
+g = C.c_void_p()
+assert ctx.lib.it_capture_end(ctx.handle, C.byref(g)) == 0
+assert len(launches()) == 1
+ctx.lib.it_graph_destroy(g)
+""")
