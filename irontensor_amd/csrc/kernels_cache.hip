@@ -125,6 +125,14 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
         }
     }
     const int s = c / 4, g = c % 4;
+    constexpr int WORDS = BITS;  // 8 channels of four tokens
+    u32x4 *vd = (u32x4 *)(region + p.c.v_off + (pb / 4) * (4 * ROW) + c * (4 * WORDS));
+    // What a block that is covered in part holds, loaded beside the new tokens rather than after their codes.
+    u32x4 old[WORDS / 4];
+    if (some && !all) {
+#pragma unroll
+        for (int q = 0; q < WORDS / 4; ++q) old[q] = vd[q];
+    }
     uint32_t vu[4][8];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -149,7 +157,6 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
         if (c == 0) *(uint16_t *)(region + p.c.vs_off + pos * 2) = f32_to_bf16_rne(vs);
     }
     if (!some) return;
-    constexpr int WORDS = BITS;  // 8 channels of four tokens
     uint32_t w[WORDS];
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
@@ -161,13 +168,11 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
             w[i] = bytes4(vu[0][i], vu[1][i], vu[2][i], vu[3][i]);
         }
     }
-    u32x4 *vd = (u32x4 *)(region + p.c.v_off + (pb / 4) * (4 * ROW) + c * (4 * WORDS));
 #pragma unroll
     for (int q = 0; q < WORDS / 4; ++q) {
         u32x4 v = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
         if (!all) {
             // the other tokens' halves (bytes) of every word stay
-            const u32x4 old = vd[q];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint32_t mine;
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(CM_THREADS) void cache_write(const CacheMoveArgs p)
                     mine = (ok[2 * (i & 1)] ? 0xffffu : 0u) | (ok[2 * (i & 1) + 1] ? 0xffff0000u : 0u);
                 else
                     mine = (ok[0] ? 0xffu : 0u) | (ok[1] ? 0xff00u : 0u) | (ok[2] ? 0xff0000u : 0u) | (ok[3] ? 0xff000000u : 0u);
-                v[i] = (v[i] & mine) | (old[i] & ~mine);
+                v[i] = (v[i] & mine) | (old[q][i] & ~mine);
             }
         }
         vd[q] = v;

@@ -46,11 +46,13 @@ def cache_values(k, v, bits):
     return stands_for(k, GROUP, levels), stands_for(v, v.shape[-1], levels)
 
 
-def attend(q, k, v, start, count, scale, capacity=None):
-    """(o, sum p|v|, largest scale * sum|q k| of a row) of q [B, n, H, D] over k, v [B, T, Hkv, D] in float64."""
+def attend(q, k, v, start, count, scale):
+    """q [B, n, H, D] over the values k, v [B, T, Hkv, D] in float64 -> (o, sum p|v|, largest scale * sum|q k| of a
+    row, sum p max|v|, largest scale * sum over the groups of max|k| sum|q|); the last two for the offsets."""
     b, n, h, d = q.shape
     t, hkv = k.shape[1:3]
-    o, pv, mag = (np.zeros(q.shape), np.zeros(q.shape), np.zeros((b, n, h)))
+    o, pv, pm = (np.zeros(q.shape) for _ in range(3))
+    mag, qm = np.zeros((b, n, h, 1)), np.zeros((b, n, h, 1))
     for bi in range(b):
         for i in range(min(n, max(0, int(count[bi])))):
             lim = min(max(int(start[bi]) + i + 1, 0), t)
@@ -64,13 +66,23 @@ def attend(q, k, v, start, count, scale, capacity=None):
                 p /= p.sum()
                 o[bi, i, hi], pv[bi, i, hi] = p @ vv, p @ np.abs(vv)
                 mag[bi, i, hi] = (np.abs(kk) @ np.abs(x)).max() * scale
-    return o, pv, mag
+                pm[bi, i, hi] = p @ np.abs(vv).max(-1)
+                qm[bi, i, hi] = (np.abs(kk).reshape(lim, -1, GROUP).max(-1) @ np.abs(x).reshape(-1, GROUP).sum(-1)).max() * scale
+    return o, pv, mag, pm, qm
 
 
-def attend_bound(o, pv, mag, t, d, bf16):
+def attend_bound(want, t, d, bf16):
     """Largest error of an element. FP32: a score is an FP32 sum of D products and D / 32 multiples of them, off by
     at most (D + 16) 2^-24 of the sum of their magnitudes; 2^x is off by 2^-21 for the sizes of x here, the
     scaled exponent's rounding among it (2^-24 |x|, |x| < 2^3 mag); a numerator and a denominator carry that,
-    and sums of T terms, each off by at most T 2^-24. BF16: P rounded (2^-8 a term) and the output (2^-8)."""
-    e = 2 * ((d + 16 + 8) * 2.0 ** -24 * mag[..., None] + 2.0 ** -21 + t * 2.0 ** -24) * pv
+    and sums of T terms, each off by at most T 2^-24. BF16: P rounded (2^-8 a term) and the output (2^-8); and
+    its sums run on codes raised by up to 24 steps (4 bits: 16 + code + 8 <= 31 steps, max|x| = 7 steps; 8 bits:
+    255 and 127), so that a sum's terms are up to 31 / 7 < 4.5 times the group's largest value, and their
+    FP32 roundings, D 2^-24 in a score and T 2^-24 in an output, go by that."""
+    o, pv, mag, pm, qm = want
+    if bf16:
+        mag = mag + 4.5 * qm
+    e = 2 * ((d + 16 + 8) * 2.0 ** -24 * mag + 2.0 ** -21 + t * 2.0 ** -24) * pv
+    if bf16:
+        e = e + 2 * (t + 2) * 2.0 ** -24 * 4.5 * pm
     return e + (2.0 ** -8 * (pv + np.abs(o) + e) if bf16 else 2.0 ** -24 * np.abs(o))
