@@ -514,8 +514,8 @@ it_status it_lion_step(it_context *ctx, int count, float *const *weights, float 
  * are deterministic.
  *
  * Quantising a group of values: step s = max|x| * (1 / L), in FP32 with 1 / L rounded, L = 7 (4 bits) or 127
- * (8 bits); codes = x / s rounded to nearest even (the real quotient's rounding); value = code * s. A step below 2^-126 is 0 and
- * the group reads as zeros; a group that holds a NaN or an infinity reads as NaN.
+ * (8 bits); codes = x / s rounded to nearest even (the real quotient's rounding); value = code * s. A step below
+ * 2^-126 is 0 and the group reads as zeros; a group that holds a NaN or an infinity reads as NaN.
  */
 
 /* A cache of `capacity` tokens of `batch` sequences with `kv_heads` heads. Keys are quantised in groups of
@@ -559,8 +559,9 @@ it_status it_kv_cache_read(it_context *ctx, it_dtype dtype, const it_kv_cache *c
  * [batch, heads, n, head_dim] contiguous or through q_layout and o_layout (NULL: q_layout), strides and
  * alignment as they come (16-byte multiples are faster). scale finite and > 0. FP32 results carry FP32
  * accuracy for the values the cache stands for; with BF16, probabilities are rounded to BF16 before their
- * product with the values. Sums run before their division by the row's sum: |v| times the positions seen
- * has to stay below 2^117. Few queries over many positions are split among blocks, with partial results in
+ * product with the values. Sums run before the steps and the row's sum are applied: |q| and max|k| times the
+ * sum of |q| have to stay below 2^112, |v| times the positions seen below 2^117; FP32 queries and values below 2^-110 keep fewer bits. O may be Q
+ * (in place, with Q's layout). Few queries over many positions are split among blocks, with partial results in
  * scratch; where the scratch cannot be had (a capture that no eager call of the size came before) they are
  * not, which takes longer and rounds differently. */
 it_status it_cached_attention(it_context *ctx, it_dtype dtype, const it_kv_cache *cache, int64_t heads, int64_t n,
@@ -574,15 +575,15 @@ it_status it_quantize_i8(it_context *ctx, it_dtype dtype, int64_t rows, int64_t 
                          int8_t *codes, int64_t ldc, float *steps);
 
 /* C[m, n] = (sum_k A[m, k] B[n, k]) steps_a[m] steps_b[n] + bias[n] in FP32 or BF16: A [M, K] and B [N, K]
- * 8-bit codes, exact 32-bit sums. K a multiple of 16 (128: faster), at most 131056; lda, ldb multiples of
- * 16, at most 4194304; codes 16-byte aligned; bias NULL: none. */
+ * 8-bit codes, exact 32-bit sums, the rest in FP32 from left to right. K a multiple of 16 (128: faster), at
+ * most 131056; lda, ldb multiples of 16, at most 4194304; codes 16-byte aligned; bias NULL: none. */
 it_status it_gemm_i8(it_context *ctx, it_dtype dtype_out, int64_t M, int64_t N, int64_t K, const int8_t *A, int64_t lda,
                      const float *steps_a, const int8_t *B, int64_t ldb, const float *steps_b, const float *bias, void *C,
                      int64_t ldc);
 
 /* A linear layer on an 8-bit weight: Y = X.W^T + bias with X [M, K] quantised per row as it_quantize_i8 does
  * (into library scratch) and W [N, K] codes from it_quantize_i8, padded with zeros to a multiple of 16, or of
- * 128 where ldw has the room. X and Y in dtype. Any K up to 130944. */
+ * 128 where ldw has the room. X and Y in dtype; Y may lie over X. Any K up to 130944. */
 it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, int64_t K, const void *X, int64_t ldx,
                        const int8_t *W, int64_t ldw, const float *steps_w, const float *bias, void *Y, int64_t ldy);
 

@@ -119,6 +119,12 @@ it_status head_layout(const char *op, const it_attn_layout *l, int64_t heads, in
     return IT_OK;
 }
 
+// Whether the address ranges of two matrices meet: `rows` rows of `cols` elements of `size` bytes.
+bool ranges_meet(const void *x, int64_t ldx, int64_t xcols, const void *y, int64_t ldy, int64_t ycols, int64_t rows, size_t size) {
+    const uintptr_t x0 = (uintptr_t)x, x1 = x0 + (size_t)((rows - 1) * ldx + xcols) * size;
+    const uintptr_t y0 = (uintptr_t)y, y1 = y0 + (size_t)((rows - 1) * ldy + ycols) * size;
+    return x0 < y1 && y0 < x1;
+}
 
 }  // namespace
 
@@ -312,7 +318,8 @@ it_status it_linear_i8(it_context *ctx, it_dtype dtype, int64_t M, int64_t N, in
         if (K > 0 && !X) return fail(IT_ERR_NULL, std::string(op) + ": NULL buffer");
         if (M > MAX_GRID) return fail(IT_ERR_DIMS, std::string(op) + ": matrix too large");
         const OnDevice dev(ctx);
-        if (it::gemv_i8_x_applicable(M, kp)) {
+        // In one launch, blocks still read X when others write Y: over X only where the codes come from scratch.
+        if (it::gemv_i8_x_applicable(M, kp) && !ranges_meet(X, ldx, K, Y, ldy, N, M, dtype == IT_BF16 ? 2 : 4)) {
             const it::GemmI8Args a{nullptr, W, nullptr, steps_w, bias, Y, M, N, kp, kp, ldw, ldy, dtype == IT_BF16, 0, 0, X, ldx, (int)K};
             return profiled(
                 ctx, [&] { return "linear_i8[" + i64(M) + "x" + i64(N) + "x" + i64(K) + "]"; },

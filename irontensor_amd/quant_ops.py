@@ -192,7 +192,7 @@ def cached_attention(q: Tensor, cache: KvCache, start: Union[Positions, Sequence
     """softmax(scale Q.K^T).V of q [batch, n, heads, head_dim] (FP32 or BF16) over the cache: query i of sequence b
     stands at position start[b] + i and sees the positions up to its own, whose tokens kv_cache_write has put
     there. heads is a multiple of the cache's heads. Queries at count[b] and beyond give zeros. scale: default
-    1 / sqrt(head_dim)."""
+    1 / sqrt(head_dim). `out` may be q itself."""
     op = "cached_attention"
     qs = _bshd(q, "Q", op)
     b, n, h, d = qs
@@ -288,7 +288,7 @@ def matmul_i8(a: Int8Matrix, b: Int8Matrix, bias: Optional[Tensor] = None, out_p
 
 def linear_i8(x: Tensor, weight: Int8Matrix, bias: Optional[Tensor] = None, *, out: Optional[Tensor] = None) -> Tensor:
     """linear (src/nn/linear.rs:87-145) on an 8-bit weight: x [.., in] (FP32 or BF16) quantised per token, times
-    weight^T, plus an FP32 bias, in x's precision."""
+    weight^T, plus an FP32 bias, in x's precision. `out` may be x itself."""
     op = "linear_i8"
     shape = x.shape()
     if not shape:

@@ -313,6 +313,20 @@ def test_padded_queries_do_not_matter(it, prec, n):
 
 
 @pytest.mark.parametrize("prec", ["f32", "bf16"])
+@pytest.mark.parametrize("n,cap", [(1, 3000), (1, 40), (70, 90)])
+def test_output_over_the_queries(it, prec, n, cap):
+    b, hkv, share, d = 2, 2, 3, 64
+    rng = np.random.default_rng(n + cap)
+    k, v = (_tensor(it, _keys(rng, (b, cap, hkv, d), prec), prec) for _ in range(2))
+    cache = it.KvCache(b, hkv, cap, d, 4)
+    it.kv_cache_write(cache, k, v, [0] * b)
+    q = _round(rng.standard_normal((b, n, hkv * share, d)), prec)
+    want = it.cached_attention(_tensor(it, q, prec), cache, [cap - n, 5]).numpy()
+    over = _tensor(it, q, prec)
+    assert np.array_equal(it.cached_attention(over, cache, [cap - n, 5], out=over).numpy(), want)
+
+
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
 def test_visible_nan_and_infinity(it, prec):
     for which in ("k", "v"):
         def fill(k, v):

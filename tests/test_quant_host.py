@@ -43,6 +43,20 @@ assert linear(0, 40, 200) == [] and attend(cache, 0, 4, pos) == []
 """)
 
 
+def test_output_over_the_input(fake):  # noqa: F811
+    """A small layer whose output meets its input takes two launches: the first has read X when the second writes Y."""
+    _run(fake, CALLS + """
+w = it.quantize_i8(it.Tensor.empty([256, 256]))
+x, y = it.Tensor.empty([4, 256]), it.Tensor.empty([4, 256])
+launches()
+it.linear_i8(x, w, out=y)
+assert len(launches()) == 1
+it.linear_i8(x, w, out=x)
+got = launches()
+assert len(got) == 2 and "quantize_rows" in got[0] and "gemv_i8" in got[1], got
+""")
+
+
 def test_refused_scratch(fake):  # noqa: F811
     """Attention runs unsplit where its scratch is refused; a layer that needs scratch says so and launches nothing."""
     _run(fake, CALLS + """

@@ -158,6 +158,18 @@ def test_linear(it, prec, m, n, k, bias):
     assert np.array_equal(both.numpy(), got)
 
 
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n", [(1, 256), (8, 512), (3, 1440), (70, 144)])
+def test_output_over_the_input(it, prec, m, n):
+    """Y in X's place, also where one launch would read X and write Y."""
+    rng = np.random.default_rng(n)
+    x = _round(rng.standard_normal((m, n)), prec)
+    layer = it.LinearI8.from_weight(it.Tensor.from_f32_slice(rng.standard_normal((n, n)), [n, n]))
+    want = layer.forward(_tensor(it, x, prec)).numpy()
+    over = _tensor(it, x, prec)
+    assert np.array_equal(layer.forward(over, out=over).numpy(), want)
+
+
 def test_rows_do_not_touch_each_other(it):
     """A NaN or infinite token makes its own row NaN, the others the same bits; 3D inputs keep their shape."""
     rng = np.random.default_rng(0)
