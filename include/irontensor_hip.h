@@ -511,7 +511,7 @@ it_status it_lion_step(it_context *ctx, int count, float *const *weights, float 
  * whose inference recomputes the whole prompt for every token and keeps weights in FP32 or BF16
  * (src/inference). All calls are stream-ordered like it_gemm, run on the context's device whatever the
  * current one is, allocate nothing but library scratch (grown once per shape, not during a capture), and
- * are deterministic.
+ * are deterministic. Work for more than one launch (2^24 blocks) is refused (IT_ERR_DIMS).
  *
  * Quantising a group of values: step s = max|x| * (1 / L), in FP32 with 1 / L rounded, L = 7 (4 bits) or 127
  * (8 bits); codes = x / s rounded to nearest even (the real quotient's rounding); value = code * s. A step below

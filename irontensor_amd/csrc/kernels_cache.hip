@@ -240,7 +240,9 @@ template <bool WRITE, typename T, int BITS>
 it_status launch_move(hipStream_t s, CacheMoveArgs a) {
     a.units = a.c.batch * a.c.kv_heads * a.blocks;  // below 2^31, checked by the caller
     const int64_t per = CM_THREADS / (a.c.head_dim / 8);
-    const dim3 grid((unsigned)((a.units + per - 1) / per)), block(CM_THREADS);
+    const int64_t blocks = (a.units + per - 1) / per;
+    if (const it_status st = check_blocks(WRITE ? "kv_cache_write" : "kv_cache_read", blocks); st != IT_OK) return st;
+    const dim3 grid((unsigned)blocks), block(CM_THREADS);
     const int d = a.c.head_dim;
     if constexpr (WRITE) {
         if (d == 64) hipLaunchKernelGGL((cache_write<T, BITS, 64>), grid, block, 0, s, a);

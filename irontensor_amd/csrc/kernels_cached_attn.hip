@@ -649,6 +649,7 @@ int64_t plan_cached_attention(CachedAttnArgs &a, bool bf16, int num_cus) {
 }
 
 it_status launch_cached_attention(hipStream_t s, bool bf16, const CachedAttnArgs &a) {
+    if (const it_status st = check_blocks("cached_attention", a.c.batch * a.c.kv_heads * a.row_blocks * a.splits); st != IT_OK) return st;
     if (bf16)
         a.c.bits == 4 ? launch_dim<false, 4>(s, a) : launch_dim<false, 8>(s, a);
     else

@@ -507,6 +507,7 @@ template <int FA, int FB, int NS>
 it_status launch_tile(hipStream_t s, GemmI8Args a) {
     a.tiles_m = (int)((a.M + 64 * FA - 1) / (64 * FA));
     a.tiles_n = (int)((a.N + 64 * FB - 1) / (64 * FB));
+    if (const it_status st = check_blocks("gemm_i8", (int64_t)a.tiles_m * a.tiles_n); st != IT_OK) return st;
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n)), block(NTHREADS);
     if (a.K % 128 == 0)
         hipLaunchKernelGGL((gemm_i8_tile<FA, FB, NS, true>), grid, block, 0, s, a);
@@ -517,27 +518,31 @@ it_status launch_tile(hipStream_t s, GemmI8Args a) {
 }
 
 template <typename T, int RL, int VN>
-void launch_rows(hipStream_t s, int64_t rows, int64_t cols, const void *X, int64_t ldx, int8_t *codes, int64_t ldc,
-                 float *steps) {
-    hipLaunchKernelGGL((quantize_rows<T, RL, VN>), dim3((unsigned)((rows + 256 / RL - 1) / (256 / RL))), dim3(256), 0, s,
-                       (const T *)X, ldx, rows, cols, std::min((cols + 127) / 128 * 128, ldc), codes, ldc, steps);
+it_status launch_rows(hipStream_t s, int64_t rows, int64_t cols, const void *X, int64_t ldx, int8_t *codes, int64_t ldc,
+                      float *steps) {
+    const int64_t blocks = (rows + 256 / RL - 1) / (256 / RL);
+    if (const it_status st = check_blocks("quantize_i8", blocks); st != IT_OK) return st;
+    hipLaunchKernelGGL((quantize_rows<T, RL, VN>), dim3((unsigned)blocks), dim3(256), 0, s, (const T *)X, ldx, rows, cols,
+                       std::min((cols + 127) / 128 * 128, ldc), codes, ldc, steps);
+    IT_HIP_TRY(hipGetLastError());
+    return IT_OK;
 }
 
 template <typename T>
-void launch_rows_of(hipStream_t s, int64_t rows, int64_t cols, const void *X, int64_t ldx, int8_t *codes, int64_t ldc,
-                    float *steps) {
+it_status launch_rows_of(hipStream_t s, int64_t rows, int64_t cols, const void *X, int64_t ldx, int8_t *codes, int64_t ldc,
+                         float *steps) {
     // A wave a row where there are rows enough to fill the GPU: no block barrier (1999 x 1237 FP32: 6.1 us with a
     // block a row, 5.6 so). Fewer rows have a block each, for the time of one row.
     if (rows >= 1024) {
-        if (cols <= 512) launch_rows<T, 64, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else if (cols <= 2048) launch_rows<T, 64, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else if (cols <= 4096) launch_rows<T, 64, 8>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else launch_rows<T, 256, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 512) return launch_rows<T, 64, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 2048) return launch_rows<T, 64, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 4096) return launch_rows<T, 64, 8>(s, rows, cols, X, ldx, codes, ldc, steps);
+        return launch_rows<T, 256, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
     } else {
-        if (cols <= 512) launch_rows<T, 64, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else if (cols <= 2048) launch_rows<T, 256, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else if (cols <= 4096) launch_rows<T, 256, 2>(s, rows, cols, X, ldx, codes, ldc, steps);
-        else launch_rows<T, 256, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 512) return launch_rows<T, 64, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 2048) return launch_rows<T, 256, 1>(s, rows, cols, X, ldx, codes, ldc, steps);
+        if (cols <= 4096) return launch_rows<T, 256, 2>(s, rows, cols, X, ldx, codes, ldc, steps);
+        return launch_rows<T, 256, 4>(s, rows, cols, X, ldx, codes, ldc, steps);
     }
 }
 
@@ -545,17 +550,14 @@ void launch_rows_of(hipStream_t s, int64_t rows, int64_t cols, const void *X, in
 
 it_status launch_quantize_i8(hipStream_t s, bool bf16, int64_t rows, int64_t cols, const void *X, int64_t ldx,
                              int8_t *codes, int64_t ldc, float *steps) {
-    if (bf16)
-        launch_rows_of<uint16_t>(s, rows, cols, X, ldx, codes, ldc, steps);
-    else
-        launch_rows_of<float>(s, rows, cols, X, ldx, codes, ldc, steps);
-    IT_HIP_TRY(hipGetLastError());
-    return IT_OK;
+    return bf16 ? launch_rows_of<uint16_t>(s, rows, cols, X, ldx, codes, ldc, steps)
+                : launch_rows_of<float>(s, rows, cols, X, ldx, codes, ldc, steps);
 }
 
 it_status launch_gemm_i8(it_context *ctx, GemmI8Args a) {
     hipStream_t s = ctx->stream;
     if (a.M <= 16) {
+        if (const it_status st = check_blocks("gemm_i8", (a.N + 15) / 16); st != IT_OK) return st;
         const dim3 grid((unsigned)((a.N + 15) / 16)), block(NTHREADS);
         if (a.M > 8)
             hipLaunchKernelGGL((gemv_i8<true>), grid, block, 0, s, a);
@@ -594,6 +596,7 @@ it_status launch_gemm_i8(it_context *ctx, GemmI8Args a) {
 bool gemv_i8_x_applicable(int64_t M, int64_t K) { return M <= 16 && M * K <= GX_MAX; }
 
 it_status launch_gemv_i8_x(hipStream_t s, bool bf16, const GemmI8Args &a) {
+    if (const it_status st = check_blocks("linear_i8", (a.N + 15) / 16); st != IT_OK) return st;
     const dim3 grid((unsigned)((a.N + 15) / 16)), block(NTHREADS);
     if (bf16)
         hipLaunchKernelGGL((gemv_i8_x<uint16_t>), grid, block, 0, s, a);

@@ -2,9 +2,18 @@
 // arguments of the launches.
 #pragma once
 
+#include <string>
+
 #include "internal.hpp"
 
 namespace it {
+
+// A launch holds fewer than 2^32 threads: at most this many blocks of 256.
+constexpr int64_t MAX_BLOCKS = 0xffffff;
+inline it_status check_blocks(const char *op, int64_t blocks) {
+    if (blocks <= MAX_BLOCKS) return IT_OK;
+    return fail(IT_ERR_DIMS, std::string(op) + ": too large for one launch, " + std::to_string((long long)blocks) + " blocks");
+}
 
 // ------------------------------------------------------------------ the cache
 

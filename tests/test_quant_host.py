@@ -57,6 +57,31 @@ assert len(got) == 2 and "quantize_rows" in got[0] and "gemv_i8" in got[1], got
 """)
 
 
+def test_launches_below_two_to_the_32_threads(fake):  # noqa: F811
+    """More blocks than a launch holds are refused, and the most that it holds are not."""
+    _run(fake, CALLS + """
+from irontensor_amd import _lib
+most, lib = 0xffffff, ctx.lib
+quantize = lambda rows, cols: lib.it_quantize_i8(ctx.handle, 0, rows, cols, 256, cols, 256, cols, 256)
+gemm = lambda m, n, k: lib.it_gemm_i8(ctx.handle, 0, m, n, k, 256, k, 256, 256, k, 256, None, 256, n)
+linear = lambda m, n, k: lib.it_linear_i8(ctx.handle, 0, m, n, k, 256, k, 256, k, 256, None, 1 << 50, n)
+def cache(units):
+    return C.byref(_lib.KvCacheDesc(4, units, 1, 4, 256, 256))  # a write touches 2 blocks of 4 tokens, 8 a thread block
+write = lambda units: lib.it_kv_cache_write(ctx.handle, 0, cache(units), 4, None, 256, 256, 256, None)
+read = lambda units: lib.it_kv_cache_read(ctx.handle, 0, cache(units), 0, 4, None, 256, 256)
+attend = lambda units: lib.it_cached_attention(ctx.handle, 0, cache(units), 1, 1, 1.0, None, None, 256, 256, None, 256)
+launches()
+for fn, args in ((quantize, (4 * most, 512)), (quantize, (most, 8192)), (gemm, (1, 16 * most, 16)), (linear, (1, 16 * most, 16)),
+                 (write, (4 * most,)), (read, (8 * most,)), (attend, (most,))):
+    assert fn(*args) == 0, (args, _lib.last_error())
+    assert len(launches()) == 1
+    over = list(args)
+    over[1 if len(args) == 3 else 0] += 1
+    assert fn(*over) == _lib.IT_ERR_DIMS and "one launch" in _lib.last_error(), (over, _lib.last_error())
+    assert launches() == []
+""")
+
+
 def test_refused_scratch(fake):  # noqa: F811
     """Attention runs unsplit where its scratch is refused; a layer that needs scratch says so and launches nothing."""
     _run(fake, CALLS + """
